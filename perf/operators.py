@@ -283,13 +283,15 @@ def _quantise(x):
 
 
 def _product(xq, xs, w, ws, k):
-    return (xq @ w[:, :k].float().t()) * xs * ws
+    """In 32 bits, which hold the sums of code products; the scales are applied
+    in 64, since what follows may be next to a border between two codes."""
+    return (xq @ w[:, :k].float().t()).double() * (xs.double() * ws.double())
 
 
 def _plain_linear(state):
     c, x = state["case"], state["x"]
     xq, xs = _quantise(x)
-    y = _product(xq, xs, state["w"], state["w_scale"], c["k"])
+    y = _product(xq, xs, state["w"], state["w_scale"], c["k"]).float()
     if state["bias"] is not None:
         y = y + state["bias"].float()
     return y.to(x.dtype)
@@ -424,15 +426,16 @@ def _exact_route(c, state):
 
 
 def _codes(x):
-    """Codes of the rows of x and their scales; a value at a border between two
-    codes is decided exactly (254 x against (2 n + 1) max: both fit 64 bits)."""
+    """Codes of the rows of x and their scales, which are 32-bit values; a value at
+    a border between two codes is decided exactly (254 x against (2 n + 1) max:
+    both fit 64 bits)."""
     x = x.double()
     most = x.abs().amax(dim=1, keepdim=True)
     safe = torch.where(most > 0, most, torch.ones_like(most))
     n = torch.floor(x * 127.0 / safe)
     twice, border = 2.0 * 127.0 * x, (2.0 * n + 1.0) * safe
     up = (twice > border) | ((twice == border) & (torch.remainder(n, 2.0) == 1.0))
-    return n + up.double(), most / 127.0
+    return n + up.double(), (most / 127.0).float().double()
 
 
 def exact(case, seed):
