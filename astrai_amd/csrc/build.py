@@ -68,6 +68,8 @@ register("moe_gemm", sources=[str(KERNELS_DIR / "moe_gemm.hip"), str(KERNELS_DIR
 register("moe_combine")
 register("moe_forward")
 register("moe_route_grad")
+register("moe_route_scores")
+register("moe_int8")
 register("capi")
 
 # The kernel names the Python loader binds (entry point astrai_<name>).

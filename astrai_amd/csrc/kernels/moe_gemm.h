@@ -280,7 +280,17 @@ int launch_route(const void* logits, int dtype, int64_t n_tokens,
                  int n_experts, int top_k, int n_shared, int32_t* topk_idx,
                  void* topk_w, int32_t* chunk_hist, hipStream_t s);
 
-// The same for at most ASTRAI_MOE_CHUNK_TOKENS tokens, straight to what
+// Routing by scores (moe_route_scores.hip): the checks of a routing (0, or the
+// error), and launch_route's outputs for one, the weights in weight_dtype.
+int check_routing(const char* who, const astrai_moe_routing* opt, int dtype,
+                  int weight_dtype, int64_t n_tokens, int n_experts, int top_k);
+int launch_route_scores(const void* logits, int dtype, const float* bias,
+                        const astrai_moe_routing& opt, int64_t n_tokens,
+                        int n_experts, int top_k, int n_shared,
+                        int weight_dtype, int32_t* topk_idx, void* topk_w,
+                        int32_t* chunk_hist, hipStream_t s);
+
+// launch_route for at most ASTRAI_MOE_CHUNK_TOKENS tokens, straight to what
 // astrai_moe_permute writes of the decisions (tiles of block_m >= 32 rows, so one
 // for every expert that has any); neither x_perm nor expert offsets.
 struct RouteList {

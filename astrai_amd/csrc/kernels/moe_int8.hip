@@ -1,0 +1,400 @@
+// Products in 8-bit integers with a scale for each token and each output channel:
+// quantisation of rows, the general product, the layer's weighted sum, and the
+// entry points of the dense product (a Linear's) and of the experts' forward.
+//
+// A row x of k values has max = max |x|, scale = max / 127 and the codes
+// q = round(127 x / max), halves to even, in [-127, 127]; a row of zeros has scale 0
+// and zero codes, one with an infinity or a NaN scale NaN and zero codes, so that
+// every product with it is NaN. Then
+//   x . w = scale_x scale_w sum_k q_x q_w
+// up to the codes' rounding, the sum in 32-bit integers: exact, in any order.
+//
+// The codes are those of the exact quotient 127 x / max (not of a rounded one), so
+// that they do not depend on how the division is carried out: a value in the
+// middle between two codes, as x = max / 2 always is, must not turn on a last bit.
+#include "moe_common.h"
+#include "moe_int8.h"
+
+namespace astrai_moe {
+namespace {
+
+// round-half-even of 127 x / max: in 64 bits 127 x is exact, and a quotient of two
+// 32-bit values cannot round onto a half it is not equal to.
+__device__ __forceinline__ int code_of(float x, double most) { return (int)rint((double)x * 127.0 / most); }
+
+// One wave per row: its maximum, then its codes, 16 at a time with the zeros
+// behind column k.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
+                                                            int64_t kp, int8_t* __restrict__ q,
+                                                            float* __restrict__ scale) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (r >= n_rows) return;
+  const T* const row = x + r * k;
+  float most = 0.0f;
+  bool bad = false;
+  for (int64_t c = lane; c < k; c += 64) {
+    const float v = fabsf(Elem<T>::to_f32(row[c]));
+    bad |= !(v < INFINITY);
+    most = fmaxf(most, v);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+  bad = __any(bad);
+  if (lane == 0) scale[r] = bad ? NAN : most / 127.0f;
+  const bool zero = bad || most == 0.0f;
+  for (int64_t c0 = lane * 16; c0 < kp; c0 += 64 * 16) {
+    union {
+      int8_t b[16];
+      uint4 v;
+    } out;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      out.b[j] = !zero && c0 + j < k ? (int8_t)code_of(Elem<T>::to_f32(row[c0 + j]), (double)most) : (int8_t)0;
+    *reinterpret_cast<uint4*>(q + r * kp + c0) = out.v;
+  }
+}
+
+// The product for every shape: 64 x 64 tiles, 64 bytes of K staged at a time, four
+// codes a multiply-add (v_dot4).
+constexpr int kTile = 64, kStep = 64, kPad = 16;
+
+template <typename T, bool kGateUp>
+__global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
+  const int tile = blockIdx.x;
+  int e = 0;
+  int64_t row0, rows;
+  if (p.tiles != nullptr) {
+    if (tile >= min(p.tiles[0], (int)min((int64_t)p.tiles[2], p.capacity))) return;
+    const int32_t* ti = p.tiles + ASTRAI_MOE_TILE_HEADER + (int64_t)tile * ASTRAI_MOE_TILE_STRIDE;
+    e = ti[0];
+    row0 = ti[1];
+    rows = min((int64_t)p.tiles[1], (int64_t)ti[2] - row0);
+  } else {
+    row0 = (int64_t)tile * p.block_m;
+    rows = min((int64_t)p.block_m, p.n_rows - row0);
+  }
+  const int64_t n0 = (int64_t)blockIdx.y * kTile;
+  const int8_t* const w0 = p.w0 + (int64_t)e * p.n * p.kp;
+  const int8_t* const w1 = kGateUp ? p.w1 + (int64_t)e * p.n * p.kp : nullptr;
+  __shared__ __attribute__((aligned(16))) int8_t As[kTile][kStep + kPad];
+  __shared__ __attribute__((aligned(16))) int8_t B0[kTile][kStep + kPad];
+  __shared__ __attribute__((aligned(16))) int8_t B1[kGateUp ? kTile : 1][kStep + kPad];
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int lr = threadIdx.x / 4, lc = threadIdx.x % 4 * 16;  // staged row and byte
+  for (int64_t rs = 0; rs < rows; rs += kTile) {
+    int acc0[4][4] = {}, acc1[4][4] = {};
+    const int64_t r = row0 + rs + lr;
+    const bool row_in = rs + lr < rows, col_in = n0 + lr < p.n;
+    const int64_t src = row_in ? (p.row_src != nullptr ? p.row_src[r] : r) : 0;
+    for (int64_t k0 = 0; k0 < p.kp; k0 += kStep) {
+      const bool k_in = k0 + lc < p.kp;
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(&As[lr][lc]) =
+          row_in && k_in ? *reinterpret_cast<const uint4*>(p.a + src * p.kp + k0 + lc) : none;
+      *reinterpret_cast<uint4*>(&B0[lr][lc]) =
+          col_in && k_in ? *reinterpret_cast<const uint4*>(w0 + (n0 + lr) * p.kp + k0 + lc) : none;
+      if (kGateUp)
+        *reinterpret_cast<uint4*>(&B1[lr][lc]) =
+            col_in && k_in ? *reinterpret_cast<const uint4*>(w1 + (n0 + lr) * p.kp + k0 + lc) : none;
+      __syncthreads();
+      for (int kk = 0; kk < kStep; kk += 4) {
+        int a[4], b0[4], b1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const int*>(&As[ty + 16 * i][kk]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          b0[j] = *reinterpret_cast<const int*>(&B0[tx + 16 * j][kk]);
+          if (kGateUp) b1[j] = *reinterpret_cast<const int*>(&B1[tx + 16 * j][kk]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc0[i][j] = __builtin_amdgcn_sdot4(a[i], b0[j], acc0[i][j], false);
+            if (kGateUp) acc1[i][j] = __builtin_amdgcn_sdot4(a[i], b1[j], acc1[i][j], false);
+          }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t in = rs + ty + 16 * i;
+      if (in >= rows) continue;
+      const int64_t row = row0 + in;
+      const float sa = p.a_scale[p.row_src != nullptr ? p.row_src[row] : row];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + tx + 16 * j;
+        if (n >= p.n) continue;
+        const float s0 = p.s0[(int64_t)e * p.n + n];
+        float v;
+        if (kGateUp) {
+          v = swiglu<T>(acc0[i][j], acc1[i][j], sa, s0, p.s1[(int64_t)e * p.n + n]);
+        } else {
+          v = (float)acc0[i][j] * (sa * s0);
+          if (p.bias != nullptr) v += Elem<T>::to_f32(static_cast<const T*>(p.bias)[n]);
+        }
+        static_cast<T*>(p.c)[row * p.n + n] = Elem<T>::from_f32(v);
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_general(const Int8Gemm& g, hipStream_t s) {
+  const int64_t cols = ceil_div(g.n, kTile);
+  ASTRAI_REQUIRE(g.capacity < (1ll << 31) && cols < 65536, "int8 product: too many tiles");
+  if (g.capacity == 0) return ASTRAI_MOE_OK;
+  hipLaunchKernelGGL((g.w1 != nullptr ? gemm_int8_kernel<T, true> : gemm_int8_kernel<T, false>),
+                     dim3((unsigned)g.capacity, (unsigned)cols), dim3(256), 0, s, g);
+  return check_launch("gemm_int8_kernel");
+}
+
+// out[t] = sum over the routed slots of w y + (sum over the shared ones of y) /
+// n_shared: 32-bit sums in the order of the slots, rounded once. A slot of weight 0
+// adds nothing, whatever its row holds (padding tokens have only such).
+template <typename T>
+__global__ __launch_bounds__(256) void sum_slots_kernel(const T* __restrict__ y, const int32_t* __restrict__ token_pos,
+                                                        const T* __restrict__ topk_w, int64_t n_tokens, int top_k,
+                                                        int n_shared, int64_t dim, T* __restrict__ out) {
+  const int64_t t = blockIdx.x;
+  const int slots = top_k + n_shared;
+  const float part = n_shared > 0 ? 1.0f / (float)n_shared : 0.0f;
+  for (int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x; c < dim; c += (int64_t)gridDim.y * 256) {
+    float sum = 0.0f;
+    for (int k = 0; k < slots; ++k) {
+      const float w = k < top_k ? Elem<T>::to_f32(topk_w[t * slots + k]) : part;
+      if (w != 0.0f) sum += w * Elem<T>::to_f32(y[(int64_t)token_pos[t * slots + k] * dim + c]);
+    }
+    out[t * dim + c] = Elem<T>::from_f32(sum);
+  }
+}
+
+int launch_sum_slots(const void* y, const int32_t* token_pos, const void* topk_w, int dtype, int64_t n_tokens,
+                     int top_k, int n_shared, int64_t dim, void* out, hipStream_t s) {
+  const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>(ceil_div(dim, 256), 64));
+  if (dtype == ASTRAI_MOE_BF16)
+    hipLaunchKernelGGL(sum_slots_kernel<bf16_t>, grid, dim3(256), 0, s, static_cast<const bf16_t*>(y), token_pos,
+                       static_cast<const bf16_t*>(topk_w), n_tokens, top_k, n_shared, dim, static_cast<bf16_t*>(out));
+  else
+    hipLaunchKernelGGL(sum_slots_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(y), token_pos,
+                       static_cast<const float*>(topk_w), n_tokens, top_k, n_shared, dim, static_cast<float*>(out));
+  return check_launch("sum_slots_kernel");
+}
+
+int check_int8(const char* who, int dtype, int64_t k, int64_t n) {
+  ASTRAI_REQUIRE(dtype == ASTRAI_MOE_BF16 || dtype == ASTRAI_MOE_F32, "%s: unsupported dtype %d", who, dtype);
+  ASTRAI_REQUIRE(k >= 1 && k <= kInt8MaxK && n >= 1 && n <= (1ll << 22),
+                 "%s: inner size must be in [1, %lld] and outputs in [1, 2^22] (got %lld, %lld)", who,
+                 (long long)kInt8MaxK, (long long)k, (long long)n);
+  return ASTRAI_MOE_OK;
+}
+
+struct Parts {  // of a workspace, 256-byte aligned
+  int64_t bytes = 0;
+  int64_t take(int64_t n) {
+    const int64_t here = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return here;
+  }
+};
+
+struct LinearPlan {
+  int64_t q, scale, bytes;
+  LinearPlan(int64_t m, int64_t k) {
+    Parts p;
+    q = p.take(m * int8_row_bytes(k));
+    scale = p.take(m * 4);
+    bytes = p.bytes;
+  }
+};
+
+struct LayerSizes {
+  int64_t n_tokens;
+  int n_experts, top_k, n_shared;
+  int64_t dim, dim_ffn;
+  int dtype;
+};
+
+int check_layer(const LayerSizes& z) {
+  if (int rc = check_int8("int8_forward", z.dtype, z.dim, z.dim_ffn)) return rc;
+  if (int rc = check_int8("int8_forward", z.dtype, z.dim_ffn, z.dim)) return rc;
+  ASTRAI_REQUIRE(z.n_shared >= 0 && z.n_shared <= ASTRAI_MOE_MAX_TOPK, "int8_forward: bad n_shared %d", z.n_shared);
+  ASTRAI_REQUIRE(z.n_experts >= 1 && z.n_experts + z.n_shared <= ASTRAI_MOE_MAX_EXPERTS,
+                 "int8_forward: n_experts + n_shared must be in [1, %d] (got %d + %d)", ASTRAI_MOE_MAX_EXPERTS,
+                 z.n_experts, z.n_shared);
+  ASTRAI_REQUIRE(z.top_k >= 1 && z.top_k <= z.n_experts && z.top_k + z.n_shared <= ASTRAI_MOE_MAX_TOPK,
+                 "int8_forward: top_k must be in [1, n_experts] and top_k + n_shared at most %d (got %d + %d)",
+                 ASTRAI_MOE_MAX_TOPK, z.top_k, z.n_shared);
+  ASTRAI_REQUIRE(z.n_tokens >= 0 && z.n_tokens * (int64_t)(z.top_k + z.n_shared) < (1ll << 31),
+                 "int8_forward: n_tokens * (top_k + n_shared) must be in [0, 2^31)");
+  return ASTRAI_MOE_OK;
+}
+
+struct LayerPlan {
+  int experts, slots, block_m;
+  int64_t rows, tiles_len, dp, fp;
+  int64_t topk_idx, topk_w, chunk_hist, chunk_base, offsets, sorted_token, sorted_w, token_pos, tiles, xq, xs, h, hq, hs,
+      y, bytes;
+  explicit LayerPlan(const LayerSizes& z) {
+    const int64_t size = z.dtype == ASTRAI_MOE_BF16 ? 2 : 4, T = z.n_tokens;
+    experts = z.n_experts + z.n_shared;
+    slots = z.top_k + z.n_shared;
+    rows = T * slots;
+    block_m = 64;
+    tiles_len = astrai_moe_tile_list_len(T, experts, slots, block_m);
+    dp = int8_row_bytes(z.dim);
+    fp = int8_row_bytes(z.dim_ffn);
+    Parts p;
+    topk_idx = p.take(rows * 4);
+    topk_w = p.take(rows * size);
+    chunk_hist = p.take(n_chunks(T) * experts * 4);
+    chunk_base = p.take(n_chunks(T) * experts * 4);
+    offsets = p.take((experts + 1) * 4);
+    sorted_token = p.take(rows * 4);
+    sorted_w = p.take(rows * size);
+    token_pos = p.take(rows * 4);
+    tiles = p.take(tiles_len * 4);
+    xq = p.take(T * dp);
+    xs = p.take(T * 4);
+    // h is read once, to be quantised, before the down product writes y
+    h = y = p.take(rows * std::max(z.dim_ffn, z.dim) * size);
+    hq = p.take(rows * fp);
+    hs = p.take(rows * 4);
+    bytes = p.bytes;
+  }
+};
+
+}  // namespace
+
+int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, float* scale, hipStream_t s) {
+  if (n_rows == 0) return ASTRAI_MOE_OK;
+  const int64_t grid = ceil_div(n_rows, 4), kp = int8_row_bytes(k);
+  if (dtype == ASTRAI_MOE_BF16)
+    hipLaunchKernelGGL(quantize_rows_kernel<bf16_t>, dim3((unsigned)grid), dim3(256), 0, s,
+                       static_cast<const bf16_t*>(x), n_rows, k, kp, q, scale);
+  else
+    hipLaunchKernelGGL(quantize_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s,
+                       static_cast<const float*>(x), n_rows, k, kp, q, scale);
+  return check_launch("quantize_rows_kernel");
+}
+
+int launch_int8_gemm(const Int8Gemm& g, hipStream_t s) {
+  return g.dtype == ASTRAI_MOE_BF16 ? launch_general<bf16_t>(g, s) : launch_general<float>(g, s);
+}
+
+}  // namespace astrai_moe
+
+using namespace astrai_moe;
+
+static bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+extern "C" int64_t astrai_moe_int8_row_bytes(int64_t k) { return k < 0 ? -1 : int8_row_bytes(k); }
+
+extern "C" int astrai_moe_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, float* scale,
+                                        void* stream) {
+  clear_error();
+  if (int rc = check_int8("quantize_rows", dtype, k, 1)) return rc;
+  ASTRAI_REQUIRE(n_rows >= 0 && n_rows < (1ll << 31), "quantize_rows: n_rows must be in [0, 2^31)");
+  if (n_rows == 0) return ASTRAI_MOE_OK;
+  ASTRAI_REQUIRE(x && q && scale, "quantize_rows: null buffer");
+  ASTRAI_REQUIRE(on16(q), "quantize_rows: q must start on a 16-byte boundary");
+  return launch_quantize_rows(x, dtype, n_rows, k, q, scale, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t astrai_moe_int8_linear_workspace_bytes(int64_t n_rows, int64_t k, int64_t n, int dtype) {
+  clear_error();
+  if (int rc = check_int8("int8_linear", dtype, k, n)) return rc;
+  ASTRAI_REQUIRE(n_rows >= 0 && n_rows < (1ll << 31), "int8_linear: n_rows must be in [0, 2^31)");
+  return LinearPlan(n_rows, k).bytes;
+}
+
+extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w, const float* w_scale,
+                                      const void* bias, int64_t n_rows, int64_t k, int64_t n, void* workspace,
+                                      int64_t workspace_bytes, void* out, void* stream) {
+  clear_error();
+  if (int rc = check_int8("int8_linear", dtype, k, n)) return rc;
+  ASTRAI_REQUIRE(n_rows >= 0 && n_rows < (1ll << 31), "int8_linear: n_rows must be in [0, 2^31)");
+  if (n_rows == 0) return ASTRAI_MOE_OK;
+  ASTRAI_REQUIRE(x && w && w_scale && workspace && out, "int8_linear: null buffer");
+  ASTRAI_REQUIRE(on16(w), "int8_linear: the weight must start on a 16-byte boundary");
+  ASTRAI_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "int8_linear: workspace must be 256-byte aligned");
+  const LinearPlan p(n_rows, k);
+  ASTRAI_REQUIRE(workspace_bytes >= p.bytes, "int8_linear: workspace holds %lld bytes, needs %lld",
+                 (long long)workspace_bytes, (long long)p.bytes);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const base = static_cast<char*>(workspace);
+  int8_t* const q = reinterpret_cast<int8_t*>(base + p.q);
+  float* const scale = reinterpret_cast<float*>(base + p.scale);
+  if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, scale, s)) return rc;
+  Int8Gemm g{};
+  g.a = q, g.a_scale = scale, g.w0 = w, g.s0 = w_scale, g.bias = bias;
+  g.kp = int8_row_bytes(k), g.n = n, g.dtype = dtype, g.c = out;
+  g.n_rows = n_rows, g.block_m = 64, g.capacity = ceil_div(n_rows, g.block_m);
+  return launch_int8_gemm(g, s);
+}
+
+extern "C" int64_t astrai_moe_int8_forward_workspace_bytes(int64_t n_tokens, int n_experts, int top_k, int n_shared,
+                                                           int64_t dim, int64_t dim_ffn, int dtype) {
+  clear_error();
+  const LayerSizes z{n_tokens, n_experts, top_k, n_shared, dim, dim_ffn, dtype};
+  if (int rc = check_layer(z)) return rc;
+  return LayerPlan(z).bytes;
+}
+
+extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* logits, int logits_dtype,
+                                       const float* bias, const astrai_moe_routing* routing, const int8_t* w_gate,
+                                       const int8_t* w_up, const int8_t* w_down, const float* gate_scale,
+                                       const float* up_scale, const float* down_scale, int64_t n_tokens, int n_experts,
+                                       int top_k, int n_shared, int64_t dim, int64_t dim_ffn, void* workspace,
+                                       int64_t workspace_bytes, void* out, void* stream) {
+  clear_error();
+  const LayerSizes z{n_tokens, n_experts, top_k, n_shared, dim, dim_ffn, dtype};
+  int rc = check_layer(z);
+  if (rc) return rc;
+  if (routing != nullptr) {
+    if ((rc = check_routing("int8_forward", routing, logits_dtype, dtype, n_tokens, n_experts, top_k))) return rc;
+  } else {
+    ASTRAI_REQUIRE(logits_dtype == dtype && bias == nullptr,
+                   "int8_forward: without a routing the logits have x's dtype and no bias");
+  }
+  if (n_tokens == 0) return ASTRAI_MOE_OK;
+  ASTRAI_REQUIRE(x && logits && w_gate && w_up && w_down && gate_scale && up_scale && down_scale && workspace && out,
+                 "int8_forward: null buffer");
+  ASTRAI_REQUIRE(on16(w_gate) && on16(w_up) && on16(w_down), "int8_forward: weights must start on 16-byte boundaries");
+  ASTRAI_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "int8_forward: workspace must be 256-byte aligned");
+  const LayerPlan p(z);
+  ASTRAI_REQUIRE(workspace_bytes >= p.bytes, "int8_forward: workspace holds %lld bytes, needs %lld",
+                 (long long)workspace_bytes, (long long)p.bytes);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const base = static_cast<char*>(workspace);
+  auto i32 = [&](int64_t off) { return reinterpret_cast<int32_t*>(base + off); };
+  auto i8 = [&](int64_t off) { return reinterpret_cast<int8_t*>(base + off); };
+  auto f32 = [&](int64_t off) { return reinterpret_cast<float*>(base + off); };
+  int32_t *const topk_idx = i32(p.topk_idx), *const hist = i32(p.chunk_hist), *const tiles = i32(p.tiles);
+  if (routing != nullptr)
+    rc = launch_route_scores(logits, logits_dtype, bias, *routing, n_tokens, n_experts, top_k, n_shared, dtype,
+                             topk_idx, base + p.topk_w, hist, s);
+  else
+    rc = launch_route(logits, dtype, n_tokens, n_experts, top_k, n_shared, topk_idx, base + p.topk_w, hist, s);
+  if (rc) return rc;
+  if ((rc = astrai_moe_permute(topk_idx, base + p.topk_w, hist, nullptr, dtype, n_tokens, p.experts, p.slots, dim,
+                               p.block_m, i32(p.offsets), i32(p.sorted_token), base + p.sorted_w, i32(p.token_pos),
+                               nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
+    return rc;
+  if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq), f32(p.xs), s))) return rc;
+  Int8Gemm g{};
+  g.a = i8(p.xq), g.a_scale = f32(p.xs), g.row_src = i32(p.sorted_token);
+  g.tiles = tiles, g.capacity = (p.tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE;
+  g.w0 = w_gate, g.w1 = w_up, g.s0 = gate_scale, g.s1 = up_scale;
+  g.kp = p.dp, g.n = dim_ffn, g.dtype = dtype, g.c = base + p.h, g.block_m = p.block_m;
+  if ((rc = launch_int8_gemm(g, s))) return rc;
+  if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq), f32(p.hs), s))) return rc;
+  g.a = i8(p.hq), g.a_scale = f32(p.hs), g.row_src = nullptr;
+  g.w0 = w_down, g.w1 = nullptr, g.s0 = down_scale, g.s1 = nullptr;
+  g.kp = p.fp, g.n = dim, g.c = base + p.y;
+  if ((rc = launch_int8_gemm(g, s))) return rc;
+  return launch_sum_slots(base + p.y, i32(p.token_pos), base + p.topk_w, dtype, n_tokens, top_k, n_shared, dim, out, s);
+}

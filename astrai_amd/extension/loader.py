@@ -30,13 +30,21 @@ import torch  # noqa: F401  (loads torch's HIP runtime before the library)
 
 KERNEL_NAMES = ["moe_route", "moe_permute", "moe_gemm_gate_up", "moe_gemm_down", "moe_combine"]
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 LIB_PATH = Path(os.environ.get("ASTRAI_MOE_LIB", Path(__file__).resolve().parent / "libastrai_moe.so"))
 
 _c_i32p = ctypes.POINTER(ctypes.c_int32)
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_f32 = ctypes.c_float
+
+
+class CRouting(ctypes.Structure):
+    """``astrai_moe_routing``."""
+
+    _fields_ = [("score", _int), ("n_groups", _int), ("topk_groups", _int), ("group_top", _int),
+                ("renormalise", _int), ("scale", _f32)]
 
 # Entry point -> argument types (mirrors include/astrai_moe.h).
 _SIGNATURES: dict[str, tuple] = {
@@ -83,6 +91,17 @@ _SIGNATURES: dict[str, tuple] = {
                                           _vp]),
     "astrai_moe_gemm_dgrad_gate_up": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _int, _i64, _int, _i64, _i64, _int, _vp,
                                              _vp, _i64, _vp]),
+    "astrai_moe_route_scores": (_int, [_vp, _int, _vp, _vp, _i64, _int, _int, _int, _vp, _vp, _vp, _vp]),
+    "astrai_moe_route_scores_grad": (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _int, _int, _vp, _vp]),
+    "astrai_moe_expert_load": (_int, [_vp, _i64, _int, _vp, _vp]),
+    "astrai_moe_balance_bias": (_int, [_vp, _vp, _int, _f32, _vp, _vp]),
+    "astrai_moe_int8_row_bytes": (_i64, [_i64]),
+    "astrai_moe_quantize_rows": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
+    "astrai_moe_int8_linear_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "astrai_moe_int8_linear": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "astrai_moe_int8_forward_workspace_bytes": (_i64, [_i64, _int, _int, _int, _i64, _i64, _int]),
+    "astrai_moe_int8_forward": (_int, [_vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int,
+                                       _int, _i64, _i64, _vp, _i64, _vp, _vp]),
     "astrai_moe_gemm_wgrad": (_int, [_vp, _vp, _vp, _int, _i64, _int, _i64, _i64, _vp, _vp]),
 }
 

@@ -21,6 +21,9 @@ Pipeline of the routed experts (``astrai/model/components/mlp.py:79-100``):
 
 from __future__ import annotations
 
+import ctypes
+import math
+from functools import lru_cache
 from typing import NamedTuple, Sequence
 
 import torch
@@ -757,3 +760,260 @@ def moe_gemm_wgrad(a: torch.Tensor, b: torch.Tensor, expert_offsets: torch.Tenso
     _lib_call("astrai_moe_gemm_wgrad", a.data_ptr(), b.data_ptr(), expert_offsets.data_ptr(), code, n_rows,
               n_experts, m, n, dw.data_ptr(), _stream(a))
     return dw
+
+
+# -- routing by scores ----------------------------------------------------------
+
+
+class Routing(NamedTuple):
+    """How a router's logits choose experts (``moe_route_scores``)."""
+
+    score: str = "softmax"  # or "sigmoid"
+    n_groups: int = 1  # groups of n_experts / n_groups consecutive experts
+    topk_groups: int = 1  # best groups whose experts may be chosen
+    group_top: int = 1  # best experts (1 or 2) whose scores make a group's value
+    renormalise: bool = True  # weights divided by their sum
+    scale: float = 1.0
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+@lru_cache(maxsize=256)
+def _check_routing(routing: Routing, n_experts: int, top_k: int) -> loader.CRouting:
+    """The library's form of a routing that suits these sizes."""
+    if routing.score not in _SCORES:
+        raise ValueError(f"unknown score {routing.score!r} (one of {sorted(_SCORES)})")
+    if not math.isfinite(routing.scale):
+        raise ValueError(f"scale must be finite, got {routing.scale}")
+    if not 1 <= n_experts <= MAX_EXPERTS:
+        raise ValueError(f"n_experts must be in [1, {MAX_EXPERTS}], got {n_experts}")
+    if not 1 <= top_k <= min(n_experts, MAX_TOPK):
+        raise ValueError(f"top_k must be in [1, min(n_experts, {MAX_TOPK})], got {top_k}")
+    groups, kept = routing.n_groups, routing.topk_groups
+    if groups < 1 or n_experts % groups or not 1 <= kept <= groups:
+        raise ValueError(f"n_groups must divide n_experts = {n_experts} and topk_groups be in [1, n_groups], "
+                         f"got {groups} and {kept}")
+    per = n_experts // groups
+    if top_k > kept * per:
+        raise ValueError(f"{kept} groups of {per} experts hold fewer than top_k = {top_k}")
+    if routing.group_top not in (1, 2) or routing.group_top > per:
+        raise ValueError(f"group_top must be 1 or 2 and at most a group's {per} experts, got {routing.group_top}")
+    return loader.CRouting(_SCORES[routing.score], groups, kept, routing.group_top, bool(routing.renormalise),
+                           routing.scale)
+
+
+def _require_like(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, like: torch.Tensor) -> None:
+    _require_gpu(t, name)
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {list(shape)} {dtype} on {like.device}, got {list(t.shape)} {t.dtype} on "
+                         f"{t.device}")
+
+
+def _launch(name: str, like: torch.Tensor, *args) -> None:
+    """Entry point ``name`` with ``like``'s device current and its current
+    stream as the last argument."""
+    fn = getattr(loader.library(), name)
+    if like.device.index == torch.cuda.current_device():
+        _check(fn(*args, _stream(like)), name)
+    else:
+        with torch.cuda.device(like.device):
+            _check(fn(*args, _stream(like)), name)
+
+
+def moe_route_scores(logits: torch.Tensor, top_k: int, routing: Routing = Routing(),
+                     bias: torch.Tensor | None = None, weight_dtype: torch.dtype | None = None) -> RouteResult:
+    """Experts by softmax or sigmoid scores, with a bias for balance (float,
+    ``[n_experts]``: it moves the choice, not the weights), groups, top-k and
+    renormalised weights of ``weight_dtype`` (default: the logits').
+
+    A logit or bias of -inf switches an expert off; slots left without one have
+    weight 0. ``astrai_moe_route_scores`` has the formulas."""
+    _require_gpu(logits, "logits", 2)
+    code = _dtype_code(logits, "logits")
+    n_tokens, n_experts = logits.shape
+    c_routing = _check_routing(routing, n_experts, top_k)
+    weight_dtype = weight_dtype or logits.dtype
+    if weight_dtype not in _DTYPE_CODES:
+        raise ValueError(f"weight_dtype must be float32 or bfloat16, got {weight_dtype}")
+    if bias is not None:
+        _require_like(bias, "bias", (n_experts,), torch.float32, logits)
+    dev = logits.device
+    topk_idx = torch.empty(n_tokens, top_k, dtype=torch.int32, device=dev)
+    topk_w = torch.empty(n_tokens, top_k, dtype=weight_dtype, device=dev)
+    chunk_hist = torch.empty(-(-n_tokens // CHUNK_TOKENS), n_experts, dtype=torch.int32, device=dev)
+    _launch("astrai_moe_route_scores", logits, logits.data_ptr(), code, _ptr(bias), ctypes.byref(c_routing), n_tokens,
+            n_experts, top_k, _DTYPE_CODES[weight_dtype], topk_idx.data_ptr(), topk_w.data_ptr(), chunk_hist.data_ptr())
+    return RouteResult(topk_idx, topk_w, chunk_hist)
+
+
+def moe_route_scores_grad(logits: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, dw: torch.Tensor,
+                          routing: Routing = Routing()) -> torch.Tensor:
+    """The logits' gradient from that of ``moe_route_scores``' weights
+    (``dw``, of their shape and type)."""
+    _require_gpu(logits, "logits", 2)
+    code = _dtype_code(logits, "logits")
+    n_tokens, n_experts = logits.shape
+    _require_gpu(topk_idx, "topk_idx", 2)
+    top_k = topk_idx.shape[1]
+    c_routing = _check_routing(routing, n_experts, top_k)
+    _require_like(topk_idx, "topk_idx", (n_tokens, top_k), torch.int32, logits)
+    weight_code = _dtype_code(topk_w, "topk_w")
+    _require_like(topk_w, "topk_w", (n_tokens, top_k), topk_w.dtype, logits)
+    _require_like(dw, "dw", (n_tokens, top_k), topk_w.dtype, logits)
+    dlogits = torch.empty_like(logits)
+    _launch("astrai_moe_route_scores_grad", logits, logits.data_ptr(), code, topk_idx.data_ptr(), topk_w.data_ptr(),
+            dw.data_ptr(), weight_code, ctypes.byref(c_routing), n_tokens, n_experts, top_k, dlogits.data_ptr())
+    return dlogits
+
+
+def moe_expert_load(chunk_hist: torch.Tensor) -> torch.Tensor:
+    """Tokens routed to each expert (int32) from a routing's ``chunk_hist``."""
+    _require_gpu(chunk_hist, "chunk_hist", 2)
+    n_chunks, n_experts = chunk_hist.shape
+    if chunk_hist.dtype != torch.int32 or not 1 <= n_experts <= MAX_EXPERTS:
+        raise ValueError(f"chunk_hist must be int32 [n_chunks, 1 .. {MAX_EXPERTS}]")
+    load = torch.empty(n_experts, dtype=torch.int32, device=chunk_hist.device)
+    _launch("astrai_moe_expert_load", chunk_hist, chunk_hist.data_ptr(), n_chunks, n_experts, load.data_ptr())
+    return load
+
+
+def moe_balance_bias(bias: torch.Tensor, load: torch.Tensor, rate: float,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """``bias + rate * sign(mean load - load)``, which draws tokens to the experts
+    that got few. ``out`` may be ``bias``; several ranks sum their loads first."""
+    _require_gpu(bias, "bias", 1)
+    n_experts = bias.shape[0]
+    if bias.dtype != torch.float32 or not 1 <= n_experts <= MAX_EXPERTS:
+        raise ValueError(f"bias must be float32 [1 .. {MAX_EXPERTS}], got {bias.dtype} {list(bias.shape)}")
+    if not math.isfinite(rate):
+        raise ValueError(f"rate must be finite, got {rate}")
+    _require_like(load, "load", (n_experts,), torch.int32, bias)
+    if out is None:
+        out = torch.empty_like(bias)
+    else:
+        _require_like(out, "out", (n_experts,), torch.float32, bias)
+    _launch("astrai_moe_balance_bias", bias, bias.data_ptr(), load.data_ptr(), n_experts, rate, out.data_ptr())
+    return out
+
+
+# -- products in 8-bit integers ---------------------------------------------------
+
+INT8_MAX_K = 131072  # longest row whose sums of code products stay below 2^31
+
+
+def int8_row_bytes(k: int) -> int:
+    """Bytes of a row of k codes: k rounded up to 16."""
+    return -(-k // 16) * 16
+
+
+def _check_int8_k(k: int, what: str) -> None:
+    if not 1 <= k <= INT8_MAX_K:
+        raise ValueError(f"{what} must be in [1, {INT8_MAX_K}], got {k}")
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """8-bit codes and scales of the rows of ``x [..., k]``: ``(q [...,
+    int8_row_bytes(k)] int8, scale [...] float32)`` with ``q = round(127 x / max
+    |x|)`` (halves to even) and ``scale = max |x| / 127``. The rows of a weight
+    ``[out, in]`` are its output channels, so this also lays out weights for
+    ``int8_linear`` and ``moe_int8_forward``."""
+    _require_gpu(x, "x")
+    code = _dtype_code(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    k, lead = x.shape[-1], x.shape[:-1]
+    _check_int8_k(k, "row length")
+    rows = math.prod(lead)
+    q = torch.empty(*lead, int8_row_bytes(k), dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    _launch("astrai_moe_quantize_rows", x, x.data_ptr(), code, rows, k, q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
+def _require_codes(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> None:
+    _require_like(t, name, shape, torch.int8, like)
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must start on a 16-byte boundary")
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x [M, K] . w^T (+ bias)`` in 8-bit integers: x's rows are quantised in
+    the call, ``w [N, int8_row_bytes(K)]`` and ``w_scale [N]`` come from
+    ``quantize_rows`` of the weight ``[N, K]``. In x's dtype, rounded once."""
+    _require_gpu(x, "x", 2)
+    code = _dtype_code(x, "x")
+    m, k = x.shape
+    _check_int8_k(k, "x's columns")
+    _require_gpu(w, "w", 2)
+    n = w.shape[0]
+    if n < 1:
+        raise ValueError("w must have at least one row")
+    _require_codes(w, "w", (n, int8_row_bytes(k)), x)
+    _require_like(w_scale, "w_scale", (n,), torch.float32, x)
+    if bias is not None:
+        _require_like(bias, "bias", (n,), x.dtype, x)
+    out = _out_buffer(out, m, n, x)
+    nbytes = loader.library().astrai_moe_int8_linear_workspace_bytes(m, k, n, code)
+    _check(0 if nbytes >= 0 else int(nbytes), "int8_linear")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _launch("astrai_moe_int8_linear", x, x.data_ptr(), code, w.data_ptr(), w_scale.data_ptr(), _ptr(bias), m, k, n,
+            ws.data_ptr(), nbytes, out.data_ptr())
+    return out
+
+
+class Int8Experts(NamedTuple):
+    """Experts' weights in 8-bit codes with a scale for each output channel
+    (``quantize_rows`` of each stack of weights), shared experts behind the
+    routed ones."""
+
+    gate: torch.Tensor  # [E, dim_ffn, int8_row_bytes(dim)] int8
+    up: torch.Tensor  # [E, dim_ffn, int8_row_bytes(dim)] int8
+    down: torch.Tensor  # [E, dim, int8_row_bytes(dim_ffn)] int8
+    gate_scale: torch.Tensor  # [E, dim_ffn] float32
+    up_scale: torch.Tensor  # [E, dim_ffn] float32
+    down_scale: torch.Tensor  # [E, dim] float32
+
+
+def moe_int8_forward(x: torch.Tensor, logits: torch.Tensor, experts: Int8Experts, top_k: int, n_shared: int = 0,
+                     routing: Routing | None = None, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """The layer's output for ``x [T, D]`` and its router logits, with the
+    experts' products in 8-bit integers, in one call of the library. ``routing``
+    (and ``bias``): as ``moe_route_scores``; None: the routing of ``moe_route``."""
+    _require_gpu(x, "x", 2)
+    _require_gpu(logits, "logits", 2)
+    code, logits_code = _dtype_code(x, "x"), _dtype_code(logits, "logits")
+    n_tokens, dim = x.shape
+    n_experts = logits.shape[1]
+    if logits.shape[0] != n_tokens or logits.device != x.device:
+        raise ValueError(f"logits must be [{n_tokens}, n_experts] on {x.device}")
+    if not 0 <= n_shared <= MAX_TOPK - top_k or n_experts + n_shared > MAX_EXPERTS:
+        raise ValueError(f"top_k + n_shared may be at most {MAX_TOPK} and n_experts + n_shared at most {MAX_EXPERTS}")
+    c_routing = None
+    if routing is not None:
+        c_routing = ctypes.byref(_check_routing(routing, n_experts, top_k))
+        if bias is not None:
+            _require_like(bias, "bias", (n_experts,), torch.float32, x)
+    elif logits.dtype != x.dtype or bias is not None:
+        raise ValueError("without a routing the logits have x's dtype and no bias")
+    elif not 1 <= top_k <= n_experts:
+        raise ValueError(f"top_k must be in [1, n_experts = {n_experts}], got {top_k}")
+    e = n_experts + n_shared
+    _require_gpu(experts.gate, "gate", 3)
+    dim_ffn = experts.gate.shape[1]
+    _check_int8_k(dim, "dim")
+    _check_int8_k(dim_ffn, "dim_ffn")
+    for name, n, k in (("gate", dim_ffn, dim), ("up", dim_ffn, dim), ("down", dim, dim_ffn)):
+        _require_codes(getattr(experts, name), name, (e, n, int8_row_bytes(k)), x)
+        _require_like(getattr(experts, name + "_scale"), name + "_scale", (e, n), torch.float32, x)
+    out = torch.empty_like(x)
+    nbytes = loader.library().astrai_moe_int8_forward_workspace_bytes(n_tokens, n_experts, top_k, n_shared, dim, dim_ffn,
+                                                                      code)
+    _check(0 if nbytes >= 0 else int(nbytes), "moe_int8_forward")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _launch("astrai_moe_int8_forward", x, x.data_ptr(), code, logits.data_ptr(), logits_code, _ptr(bias), c_routing,
+            experts.gate.data_ptr(), experts.up.data_ptr(), experts.down.data_ptr(), experts.gate_scale.data_ptr(),
+            experts.up_scale.data_ptr(), experts.down_scale.data_ptr(), n_tokens, n_experts, top_k, n_shared, dim,
+            dim_ffn, ws.data_ptr(), nbytes, out.data_ptr())
+    return out

@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define ASTRAI_MOE_ABI_VERSION 11
+#define ASTRAI_MOE_ABI_VERSION 12
 
 /* Element types. */
 #define ASTRAI_MOE_F32 0
@@ -518,6 +518,143 @@ int astrai_moe_gemm_wgrad(const void* a, const void* b,
                           const int32_t* expert_offsets, int dtype,
                           int64_t n_rows, int n_experts, int64_t m, int64_t n,
                           void* dw, void* stream);
+
+/*
+ * Routing by scores. No counterpart in the reference, whose router knows
+ * softmax scores only (mlp.py:84-87, astrai_moe_route): softmax or sigmoid
+ * scores, a bias for balance, groups of experts, renormalised or plain weights
+ * and a scale. For a token with logits l:
+ *   s = softmax(l) or sigmoid(l) over all experts
+ *   c_e = s_e + bias_e (bias NULL: s_e); -inf where l_e or bias_e is -inf or
+ *     bias_e is NaN: an expert switched off
+ *   the experts form n_groups groups of n_experts / n_groups consecutive ones; a
+ *     group's value is the sum of its group_top (1 or 2) largest c, and the
+ *     topk_groups groups of the largest values stay (ties: the lower group)
+ *   topk_idx: the top_k largest c among these, descending (ties: the lower
+ *     expert); slots without a c above -inf left take the lowest experts not yet
+ *     chosen and weight 0
+ *   topk_w = scale s / S over the chosen s, S their sum (0 where S = 0), or with
+ *     renormalise 0 scale s; rounded once to weight_dtype
+ * The choice is made in 64 bits. A row with a NaN logit (softmax: or +inf) has
+ * experts 0 .. top_k - 1 and NaN weights.
+ *
+ *   logits     [n_tokens, n_experts]  dtype
+ *   bias       [n_experts]            float, or NULL
+ *   routing    on the host, read before the call returns
+ *   topk_idx, topk_w (weight_dtype), chunk_hist   as astrai_moe_route writes
+ */
+#define ASTRAI_MOE_SCORE_SOFTMAX 0
+#define ASTRAI_MOE_SCORE_SIGMOID 1
+typedef struct astrai_moe_routing {
+  int score;       /* ASTRAI_MOE_SCORE_* */
+  int n_groups;    /* divides n_experts; 1: no groups */
+  int topk_groups; /* in [1, n_groups], holding at least top_k experts */
+  int group_top;   /* 1 or 2, at most a group's experts */
+  int renormalise;
+  float scale;     /* finite */
+} astrai_moe_routing;
+int astrai_moe_route_scores(const void* logits, int dtype, const float* bias,
+                            const astrai_moe_routing* routing,
+                            int64_t n_tokens, int n_experts, int top_k,
+                            int weight_dtype, int32_t* topk_idx, void* topk_w,
+                            int32_t* chunk_hist, void* stream);
+
+/*
+ * Gradient of the logits from dw, that of astrai_moe_route_scores' weights, at
+ * the chosen experts, in float with one rounding to dtype. Slots of weight 0 have
+ * no part in it; the bias gets no gradient (it moves the choice only).
+ *   topk_idx, topk_w  as astrai_moe_route_scores wrote them
+ *   dw                [n_tokens, top_k]      weight_dtype
+ *   dlogits           [n_tokens, n_experts]  dtype
+ */
+int astrai_moe_route_scores_grad(const void* logits, int dtype,
+                                 const int32_t* topk_idx, const void* topk_w,
+                                 const void* dw, int weight_dtype,
+                                 const astrai_moe_routing* routing,
+                                 int64_t n_tokens, int n_experts, int top_k,
+                                 void* dlogits, void* stream);
+
+/* load[e]: tokens routed to expert e, from the chunks' histograms [n_chunks, n_experts]. */
+int astrai_moe_expert_load(const int32_t* chunk_hist, int64_t n_chunks,
+                           int n_experts, int32_t* load, void* stream);
+
+/* out[e] = bias[e] + rate * sign(mean load - load[e]); out may be bias. */
+int astrai_moe_balance_bias(const float* bias, const int32_t* load,
+                            int n_experts, float rate, float* out,
+                            void* stream);
+
+/*
+ * Products in 8-bit integers, with a scale for each token (taken from the
+ * activations) and each output channel of a weight (no counterpart in the
+ * reference). A row x of k values has the codes round(127 x / max |x|), halves
+ * to even, and the scale max |x| / 127; a row of zeros has codes and scale 0, one
+ * with an infinity or a NaN codes 0 and scale NaN, which makes its products NaN.
+ * The codes of a row take astrai_moe_int8_row_bytes(k) bytes, k rounded up to
+ * 16; those of activations are 0 behind column k, those of weights may be
+ * anything. Sums of code products are exact 32-bit integers: k up to 131072.
+ *
+ *   x      [n_rows, k]                 dtype
+ *   q      [n_rows, row_bytes(k)]      int8, 16-byte aligned
+ *   scale  [n_rows]                    float
+ */
+int64_t astrai_moe_int8_row_bytes(int64_t k);
+int astrai_moe_quantize_rows(const void* x, int dtype, int64_t n_rows,
+                             int64_t k, int8_t* q, float* scale, void* stream);
+
+/*
+ * out = x . w^T + bias with x's rows quantised as above: out[m, n] = scale_m
+ * w_scale[n] sum_k q[m, k] w[n, k] + bias[n], rounded once to dtype (a Linear's
+ * product, linear.py:23-24, with an int8 weight).
+ *   x          [n_rows, k]              dtype
+ *   w          [n, row_bytes(k)]        int8, 16-byte aligned
+ *   w_scale    [n]                      float
+ *   bias       [n]                      dtype, or NULL
+ *   workspace  astrai_moe_int8_linear_workspace_bytes(...) bytes for the same
+ *              sizes, 256-byte aligned, nothing to initialise; calls sharing one
+ *              must not overlap
+ *   out        [n_rows, n]              dtype
+ */
+int64_t astrai_moe_int8_linear_workspace_bytes(int64_t n_rows, int64_t k,
+                                               int64_t n, int dtype);
+int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
+                           const float* w_scale, const void* bias,
+                           int64_t n_rows, int64_t k, int64_t n,
+                           void* workspace, int64_t workspace_bytes, void* out,
+                           void* stream);
+
+/*
+ * astrai_moe_forward with int8 expert weights: from the router's logits to the
+ * layer's output. Each expert is the SwiGLU MLP in 8-bit integers: the token's
+ * row quantised, g and u its products with the gate and up weights, h =
+ * round(silu(g) u) to dtype, h quantised, y = round(its product with the down
+ * weight) to dtype. The output is the sum over the token's routed experts of w y
+ * plus the mean over the shared ones of y, in float, rounded once; a slot of
+ * weight 0 adds nothing.
+ *   routing    as astrai_moe_route_scores' (bias: its bias), or NULL: the
+ *              reference's routing, astrai_moe_route (logits of x's dtype, no bias)
+ *   w_gate, w_up    [n_experts + n_shared, dim_ffn, row_bytes(dim)]   int8
+ *   w_down          [n_experts + n_shared, dim, row_bytes(dim_ffn)]   int8, all
+ *              16-byte aligned, the shared experts behind the routed ones
+ *   gate_scale, up_scale  [n_experts + n_shared, dim_ffn] float
+ *   down_scale            [n_experts + n_shared, dim]     float
+ *   workspace  astrai_moe_int8_forward_workspace_bytes(...) bytes for the same
+ *              sizes, 256-byte aligned, nothing to initialise; calls sharing one
+ *              must not overlap
+ */
+int64_t astrai_moe_int8_forward_workspace_bytes(int64_t n_tokens, int n_experts,
+                                                int top_k, int n_shared,
+                                                int64_t dim, int64_t dim_ffn,
+                                                int dtype);
+int astrai_moe_int8_forward(const void* x, int dtype, const void* logits,
+                            int logits_dtype, const float* bias,
+                            const astrai_moe_routing* routing,
+                            const int8_t* w_gate, const int8_t* w_up,
+                            const int8_t* w_down, const float* gate_scale,
+                            const float* up_scale, const float* down_scale,
+                            int64_t n_tokens, int n_experts, int top_k,
+                            int n_shared, int64_t dim, int64_t dim_ffn,
+                            void* workspace, int64_t workspace_bytes,
+                            void* out, void* stream);
 
 #ifdef __cplusplus
 }
