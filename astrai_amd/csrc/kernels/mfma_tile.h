@@ -213,6 +213,70 @@ struct SplitWalk : TileWalk<GM> {
   }
 };
 
+// The order in which one workgroup takes its work items. Items below `dyn`
+// are dealt statically: the workgroup's slot, then every G-th item. Given a
+// scheduling block (`sched`, its counter cleared before the launch), the
+// items from `dyn` on are claimed at run time from the counter sched[0] by
+// whichever workgroups get there first, so that the compute units running at
+// a higher clock take more of them (the XCDs of one part hold clocks several
+// per cent apart under this load, and with a static deal the slowest one sets
+// the kernel's end). Matrix-core wave 0 claims a workgroup's next item
+// kClaimLead steps before the end of its current one and publishes it in the
+// workgroup's ring of 8 mailbox slots (sched[kMailboxBase + 8 b ...]); every
+// wave reads it when it leaves the current item, at least two barriers
+// after the store (the DMA waves run up to three steps ahead of the
+// matrix-core waves). -1: no item. Claiming that late needs every dynamic
+// item to last more than kClaimLead steps. A claim stalls its workgroup for
+// about an atomic's round trip, so claims are made only where tiles are long
+// (kDynamicMinSteps): measured against the static deal, in one process with
+// the builds alternating, the Mixtral-shaped GEMMs (64 and 224 steps per
+// tile) gained 1.8 % (gate/up) and 0.8 % (down). At the fine-grained shape
+// the 32-step gate/up tiles gained 2.3-2.7 % (1.1-1.2 % with the skewed
+// router) once padding-only waves idled, and the 22-step down tiles lost
+// 1.3-1.7 %.
+constexpr int kMailboxBase = 64;       // int32 offset of the mailboxes in the scheduling block
+constexpr int kMaxSchedGroups = 1024;  // workgroups the scheduling block has mailboxes for
+constexpr int kDynamicShare = 10;      // 1 / kDynamicShare of the items are claimed at run time
+constexpr int kDynamicMinSteps = 32;   // K steps per tile from which items are claimed at run time
+constexpr int kClaimLead = 6;
+static_assert(kClaimLead > 4 && kClaimLead < kSplitMinSteps, "claim between the DMA waves' lead and an item's end");
+
+struct ItemSeq {
+  int slot, G, m, n, dyn;
+  int* mbox;  // the workgroup's 8 mailbox slots (nullptr: static deal only)
+  template <int GM>
+  __device__ ItemSeq(const SplitWalk<GM>& walk, int KT, int* sched)
+      : slot(walk.first_slot()), G(walk.G), n(walk.items()), dyn(walk.items()), mbox(nullptr) {
+    if (sched != nullptr && KT >= kDynamicMinSteps && G <= kMaxSchedGroups) {
+      const int d = max(G, n - n / kDynamicShare);
+      if (d < n) dyn = d, mbox = sched + kMailboxBase + 8 * (int)blockIdx.x;
+    }
+    m = slot < dyn ? (dyn - slot + G - 1) / G : 0;
+  }
+  // the workgroup's item `idx` (a mailbox read for the claimed ones)
+  __device__ int id(int idx) const {
+    if (idx < m) return slot + idx * G;
+    if (mbox == nullptr) return -1;
+    return __builtin_amdgcn_readfirstlane(
+        __hip_atomic_load(mbox + ((idx - m) & 7), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  }
+  // whether the item after `idx` is claimed at run time
+  __device__ bool claims_next(int idx) const { return mbox != nullptr && idx + 1 >= m; }
+  // matrix-core wave 0, kClaimLead steps before the end of item `idx`:
+  // claims the next item; false once a claim came back empty
+  __device__ bool claim(int idx, int* sched) const {
+    int c = 0;
+    if (__lane_id() == 0) c = __hip_atomic_fetch_add(sched, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    c = __builtin_amdgcn_readfirstlane(c);
+    const int v = dyn + c < n ? dyn + c : -1;
+    if (__lane_id() == 0)
+      __hip_atomic_store(mbox + ((idx + 1 - m) & 7), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // the store lands in L2 before this wave's next barrier
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    return v >= 0;
+  }
+};
+
 // A tail unit's fp32 accumulators, wave by wave in the accumulator layout:
 // part[unit][wave][i][j][lane] as 16-byte vectors (one 1 KB store per wave
 // and 16x16 tile).
