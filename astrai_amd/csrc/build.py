@@ -69,7 +69,8 @@ register("moe_combine")
 register("moe_forward")
 register("moe_route_grad")
 register("moe_route_scores")
-register("moe_int8")
+register("moe_int8", sources=[str(KERNELS_DIR / "moe_int8.hip"), str(KERNELS_DIR / "moe_gemm_int8.hip"),
+                              str(KERNELS_DIR / "moe_gemm_int8_ragged.hip")])
 register("capi")
 
 # The kernel names the Python loader binds (entry point astrai_<name>).

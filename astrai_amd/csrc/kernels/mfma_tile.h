@@ -137,6 +137,9 @@ struct TileWalk {
         n_live(min(tiles[0], min(tiles[2], capacity))),
         total(n_live * n_tiles_n),
         group_size(GM * n_tiles_n) {}
+  // n_live_ row tiles known without a list
+  __device__ TileWalk(int n_live_, int n_tiles_n)
+      : G((int)gridDim.x), n_live(n_live_), total(n_live_ * n_tiles_n), group_size(GM * n_tiles_n) {}
   __device__ int first_slot() const {
     const int bid = blockIdx.x;
     return (G % kXcds == 0) ? (bid % kXcds) * (G / kXcds) + bid / kXcds : bid;

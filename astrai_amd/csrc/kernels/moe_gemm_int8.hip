@@ -1,0 +1,507 @@
+// 8-bit integer products on CDNA4 matrix cores (gfx950): the grouped gate/up and
+// down products of int8 experts and a Linear's dense product.
+//
+// v_mfma_i32_16x16x64_i8 takes 16 consecutive codes of a row per lane where
+// v_mfma_f32_16x16x32_bf16 takes 8 bf16 values: the same 16 bytes, in the same
+// time, for twice the products. A row of kp codes is therefore staged, swizzled
+// and read like a bf16 row of kp / 2 values (mfma_tile.h), a K step is 128 codes,
+// and the tiles, the walk and the waves' roles are those of moe_gemm_mfma.hip;
+// only the sums (32-bit integers, exact in any order) and the epilogue differ:
+//   sum * (scale of the row * scale of the column) (+ bias), or
+//   silu(g) u of two such products,
+// rounded once to the output's type. Sums being exact, every tile, split and order
+// gives the same bits.
+#include <algorithm>
+#include <cmath>
+
+#include "mfma_pick.h"
+#include "mfma_tile.h"
+#include "moe_int8.h"
+
+#include <type_traits>
+
+// Set to 1 by moe_gemm_int8_ragged.hip, which builds these kernels a second time
+// for rows that are no whole number of 128-byte steps, or outputs whose rows are no
+// whole number of 16-byte stores.
+#ifndef ASTRAI_MOE_RAGGED_K
+#define ASTRAI_MOE_RAGGED_K 0
+#endif
+
+namespace astrai_moe {
+namespace {
+
+constexpr bool kRagged = ASTRAI_MOE_RAGGED_K != 0;
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+// The row tiles of a launch: those of the list, or one expert's n_rows rows.
+struct RowTiles {
+  const int32_t* tiles;
+  int n_rows, block_m;
+  __device__ int live(int capacity) const {
+    return tiles == nullptr ? capacity : min(tiles[0], min(tiles[2], capacity));
+  }
+  __device__ void get(int mt, int& e, int& row0, int& end) const {
+    if (tiles == nullptr) {
+      e = 0;
+      row0 = mt * block_m;
+      end = n_rows;
+    } else {
+      const int32_t* ti = tiles + ASTRAI_MOE_TILE_HEADER + (int64_t)mt * ASTRAI_MOE_TILE_STRIDE;
+      e = ti[0];
+      row0 = ti[1];
+      end = ti[2];
+    }
+  }
+};
+
+struct Args {
+  const int8_t* a;
+  const float* a_scale;
+  const int32_t* row_src;
+  RowTiles tiles;
+  const int8_t *w0, *w1;
+  const float *s0, *s1;
+  const void* bias;
+  int kp, n, n_tiles_n, capacity;
+  void* c;
+  float* part;     // partial sums of a split last round, or null
+  int32_t* sched;  // run-time claims, or null
+};
+
+// Per-tile global bases (bytes).
+template <int BM, int BN, bool kGateUp, bool kGather>
+struct I8Src {
+  const char* a_base = nullptr;
+  const char* b_base0 = nullptr;
+  const char* b_base1 = nullptr;
+  int e = 0, row0 = 0, rows = 0, b_rows = 0;
+  __device__ void setup(const Args& p, int mt, int nt, int row_off = 0) {
+    int end;
+    p.tiles.get(mt, e, row0, end);
+    row0 += row_off;
+    rows = min(BM, end - row0);
+    constexpr int kTileRows = kGateUp ? BN / 2 : BN;
+    b_rows = min(kTileRows, p.n - nt * kTileRows);
+    a_base = reinterpret_cast<const char*>(kGather ? p.a : p.a + (int64_t)row0 * p.kp);
+    const int64_t at = ((int64_t)e * p.n + (int64_t)nt * kTileRows) * p.kp;
+    b_base0 = reinterpret_cast<const char*>(p.w0 + at);
+    b_base1 = kGateUp ? reinterpret_cast<const char*>(p.w1 + at) : b_base0;
+  }
+  template <bool kTail>
+  __device__ void dma_a_rows(const DmaLane& dl, uint32_t row_off, int q, uint32_t kp, char* lds) const {
+    if constexpr (kTail)
+      dma_16_or_zero(a_base, row_off + dl.chunk(q), dl.chunk(q), kp, lds);
+    else
+      lds_dma_16(a_base + (row_off + dl.chunk(q)), lds);
+  }
+  template <bool kTail>
+  __device__ void dma_b(const DmaLane& dl, int q, uint32_t kp, char* lds) const {
+    const int r0 = q * 8;
+    const char* bb = (kGateUp && r0 >= BN / 2) ? b_base1 : b_base0;
+    const int rq = (kGateUp && r0 >= BN / 2) ? r0 - BN / 2 : r0;
+    const uint32_t off = (uint32_t)min(rq + dl.row, b_rows - 1) * kp + dl.chunk(q);
+    if constexpr (kTail)
+      dma_16_or_zero(bb, off, dl.chunk(q), kp, lds);
+    else
+      lds_dma_16(bb + off, lds);
+  }
+};
+
+// Byte offsets of the activation rows one lane loads in its NQ DMA ops of a tile
+// (pad rows re-read the tile's last row), gathered through row_src or not. Gathered
+// rows lie anywhere in a (under 4 GiB), others behind the tile's first.
+template <int NQ, bool kGather>
+struct RowOffsets {
+  uint32_t off[NQ];
+  __device__ void load(const int32_t* row_src, int row0, int rows, int qbase, int lane, uint32_t kp) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int r = min((qbase + i) * 8 + (lane >> 3), rows - 1);
+      off[i] = (kGather ? (uint32_t)row_src[row0 + r] : (uint32_t)r) * kp;
+    }
+  }
+};
+
+__device__ __forceinline__ float scale_of(const Args& p, bool gather, int row) {
+  return p.a_scale[gather ? p.row_src[row] : row];
+}
+
+// The scales of four columns of expert e from column n on; columns past the
+// matrix get 0.
+__device__ __forceinline__ f32x4_t four(const float* s, int64_t e, int n, int n_all) {
+  typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));  // (scales start anywhere)
+  const float* const at = s + e * n_all + n;
+  if (!kRagged) return n < n_all ? (f32x4_t)*reinterpret_cast<const f32x4_u*>(at) : f32x4_t{0, 0, 0, 0};
+  f32x4_t v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = n + r < n_all ? at[r] : 0.0f;
+  return v;
+}
+
+template <typename T>
+struct Out4 {
+  typedef bf16x4_t type;
+};
+template <>
+struct Out4<float> {
+  typedef f32x4_t type;
+};
+
+// Four output values of a lane: columns n .. n + 3 of a row.
+template <typename T, bool kGateUp>
+__device__ __forceinline__ typename Out4<T>::type out_of(const i32x4_t& g, const i32x4_t& u, float sa, const f32x4_t& s0,
+                                                         const f32x4_t& s1, const f32x4_t& bias) {
+  typename Out4<T>::type o;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float v;
+    if constexpr (kGateUp)
+      v = swiglu<T>(g[r], u[r], sa, s0[r], s1[r]);
+    else
+      v = (float)g[r] * (sa * s0[r]) + bias[r];
+    if constexpr (std::is_same_v<T, bf16_t>)
+      o[r] = (__bf16)v;
+    else
+      o[r] = v;
+  }
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4_t bias_of(const void* bias, int n, int n_all) {
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (bias != nullptr)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < n_all) v[r] = Elem<T>::to_f32(static_cast<const T*>(bias)[n + r]);
+  return v;
+}
+
+// The epilogue of one wave's WM x WN sums: the accumulator layout gives lane l
+// columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile. bf16 outputs are
+// transposed in pairs of tiles to 16-byte stores; fp32 ones are 16 bytes as they
+// lie. Outputs whose rows are no whole number of 16 bytes are stored by element.
+template <typename T, bool kGateUp, int WM, int WN, int BN>
+__device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16], const Args& p, bool gather, int e,
+                                           int wm, int wn, int t_row0, int t_rows, int t_nt) {
+  constexpr int MT16 = WM / 16, NT16 = WN / 16, NJ = kGateUp ? NT16 / 2 : NT16;
+  static_assert(NJ % 2 == 0, "tiles are stored in pairs");
+  const int el = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  const int row_l = el & 15, q = el >> 4;
+  const int n_base = kGateUp ? t_nt * (BN / 2) + wn * (WN / 2) : t_nt * BN + wn * WN;
+  const int N = p.n;
+  T* const C = static_cast<T*>(p.c);
+  const bool whole = !kRagged || (N * (int)sizeof(T)) % 16 == 0;
+  float sa[MT16];
+#pragma unroll
+  for (int i = 0; i < MT16; ++i) sa[i] = scale_of(p, gather, t_row0 + min(wm * WM + i * 16 + row_l, t_rows - 1));
+#pragma unroll
+  for (int jp = 0; jp < NJ; jp += 2) {
+    f32x4_t s0[2], s1[2], b[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int n = n_base + (jp + h) * 16 + 4 * q;
+      s0[h] = four(p.s0, e, n, N);
+      if constexpr (kGateUp) s1[h] = four(p.s1, e, n, N);
+      b[h] = kGateUp ? f32x4_t{0, 0, 0, 0} : bias_of<T>(p.bias, n, N);
+    }
+#pragma unroll
+    for (int i = 0; i < MT16; ++i) {
+      const int gm = wm * WM + i * 16 + row_l;
+      const int64_t row_off = (int64_t)(t_row0 + min(gm, t_rows - 1)) * N;
+      typename Out4<T>::type o[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o[h] = out_of<T, kGateUp>(acc[i][jp + h], acc[i][kGateUp ? jp + h + NJ : jp + h], sa[i], s0[h], s1[h], b[h]);
+      if (whole) {
+        if constexpr (std::is_same_v<T, bf16_t>) {
+          transpose2(o);
+          const int n = n_base + jp * 16 + 8 * q;
+          bf16x8_t v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = o[0][r], v[4 + r] = o[1][r];
+          if (gm < t_rows && n < N) *reinterpret_cast<bf16x8_t*>(C + row_off + n) = v;
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int n = n_base + (jp + h) * 16 + 4 * q;
+            if (gm < t_rows && n < N) *reinterpret_cast<f32x4_t*>(C + row_off + n) = o[h];
+          }
+        }
+      } else if (gm < t_rows) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int n = n_base + (jp + h) * 16 + 4 * q;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < N) {
+              using E = std::conditional_t<std::is_same_v<T, bf16_t>, __bf16, T>;
+              reinterpret_cast<E*>(C)[row_off + n + r] = o[h][r];
+            }
+        }
+      }
+    }
+  }
+}
+
+// ===========================================================================
+// 32-, 64- and 128-row tiles: every wave issues DMA, several stages in flight.
+// ===========================================================================
+template <int BM_, int BN_, int STAGES_, int WGM_, int WGN_, int GM_>
+struct TileCfg {
+  static constexpr int BM = BM_, BN = BN_, STAGES = STAGES_, WGM = WGM_, WGN = WGN_, GM = GM_;
+  static constexpr int WAVES = WGM * WGN;
+  static constexpr int THREADS = WAVES * 64;
+  static constexpr int WM = BM / WGM;  // rows per wave
+  static constexpr int WN = BN / WGN;  // columns per wave
+  static constexpr int A_BYTES = BM * kRowBytes;
+  static constexpr int B_BYTES = BN * kRowBytes;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int A_PER_WAVE = A_BYTES / 1024 / WAVES;  // 1 KB DMA ops per wave
+  static constexpr int B_PER_WAVE = B_BYTES / 1024 / WAVES;
+  static constexpr int DMA_PER_WAVE = A_PER_WAVE + B_PER_WAVE;
+  static_assert(A_BYTES % (1024 * WAVES) == 0 && B_BYTES % (1024 * WAVES) == 0, "DMA ops split over waves");
+  static_assert(WM % 16 == 0 && WN % 32 == 0, "16x16 MFMA tiles; gate/up halves");
+  static_assert(STAGES >= 2 && STAGES * STAGE_BYTES <= 160 * 1024, "LDS");
+  static_assert(DMA_PER_WAVE * (STAGES - 1) <= 63, "vmcnt range");
+};
+
+// kHalves: the list holds 256-row tiles, each walked as two of 128 rows.
+template <typename Cfg, typename T, bool kGateUp, bool kGather, bool kHalves>
+__global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(const Args p) {
+  constexpr int S = Cfg::STAGES;
+  constexpr int DPW = Cfg::DMA_PER_WAVE;
+  __shared__ __attribute__((aligned(1024))) char smem[S * Cfg::STAGE_BYTES];
+  static_assert(!kHalves || Cfg::BM == 128, "halves of 256-row tiles");
+  const TileWalk<Cfg::GM> walk(p.tiles.live(p.capacity), kHalves ? 2 * p.n_tiles_n : p.n_tiles_n);
+  int mt = 0, nt = 0;
+  // the workgroup's first tile from `logical` on that has rows (a tile of at
+  // most 128 rows has no second half)
+  auto seek = [&](int logical_, int& mt_, int& nt_) {
+    int at = walk.seek(logical_, mt_, nt_);
+    if constexpr (kHalves) {
+      while (at < walk.total && (nt_ & 1) != 0) {
+        int e, row0, end;
+        p.tiles.get(mt_, e, row0, end);
+        if (row0 + 128 < end) break;
+        at = walk.seek(at + walk.G, mt_, nt_);
+      }
+    }
+    return at;
+  };
+  int logical = seek(walk.first_slot(), mt, nt);
+  if (logical >= walk.total) return;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wm = wave / Cfg::WGN;
+  const int wn = wave % Cfg::WGN;
+  const uint32_t kp = (uint32_t)p.kp;
+  I8Src<Cfg::BM, Cfg::BN, kGateUp, kGather> src;
+  RowOffsets<Cfg::A_PER_WAVE, kGather> rows;
+  const int KT = (int)((kp + kRowBytes - 1) / kRowBytes);
+  // K steps start at step (7 e) mod KT, so that workgroups streaming different
+  // experts read their weight rows at different offsets (as in moe_gemm_mfma.hip)
+  int k_start = 0;
+  auto setup_tile = [&](int mt_, int nt_) {
+    if constexpr (kHalves)
+      src.setup(p, mt_, nt_ >> 1, (nt_ & 1) * 128);
+    else
+      src.setup(p, mt_, nt_);
+    k_start = (src.e * 7) % KT;
+    rows.load(p.row_src, src.row0, src.rows, wave * Cfg::A_PER_WAVE, lane, kp);
+  };
+  auto stage_ops = [&](auto tail_c, int ks, int buf) {
+    constexpr bool kTail = decltype(tail_c)::value;
+    char* sa = smem + buf * Cfg::STAGE_BYTES;
+    char* sb = sa + Cfg::A_BYTES;
+    const DmaLane dl(lane, ks);
+#pragma unroll
+    for (int i = 0; i < Cfg::A_PER_WAVE; ++i) {
+      const int q = wave * Cfg::A_PER_WAVE + i;
+      src.template dma_a_rows<kTail>(dl, rows.off[i], q, kp, sa + q * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < Cfg::B_PER_WAVE; ++i) {
+      const int q = wave * Cfg::B_PER_WAVE + i;
+      src.template dma_b<kTail>(dl, q, kp, sb + q * 1024);
+    }
+  };
+  auto issue_stage = [&](int kstep, int buf) {  // the tile's kstep-th step
+    const int ks = kstep + k_start < KT ? kstep + k_start : kstep + k_start - KT;  // K step loaded
+    if (kRagged && (uint32_t)(ks + 1) * kRowBytes > kp)
+      stage_ops(std::true_type{}, ks, buf);
+    else
+      stage_ops(std::false_type{}, ks, buf);
+  };
+
+  // ---- fragment reads (16x16x64: lane l holds row l % 16, codes 16 (l / 16) .. + 15) ----
+  constexpr int MT16 = Cfg::WM / 16, NT16 = Cfg::WN / 16;
+  const int frag_row = lane & 15;
+  const int fq = lane >> 4;
+  const int fsw = (frag_row >> 1) & 7;  // row bases are multiples of 16
+  int a_off[MT16];
+#pragma unroll
+  for (int i = 0; i < MT16; ++i) a_off[i] = (wm * Cfg::WM + i * 16 + frag_row) * kRowBytes;
+  int b_off[NT16];
+#pragma unroll
+  for (int j = 0; j < NT16; ++j) {
+    int r;
+    if (kGateUp) {
+      constexpr int half = NT16 / 2;
+      r = (j < half) ? wn * (Cfg::WN / 2) + j * 16 : Cfg::BN / 2 + wn * (Cfg::WN / 2) + (j - half) * 16;
+    } else {
+      r = wn * Cfg::WN + j * 16;
+    }
+    b_off[j] = (r + frag_row) * kRowBytes;
+  }
+  i32x4_t fa[2][MT16], fb[2][NT16];
+  auto read_frags = [&](int buf, int kh, int slot_) {
+    const char* sa = smem + buf * Cfg::STAGE_BYTES;
+    const char* sb = sa + Cfg::A_BYTES;
+    const int sw = ((kh * 4 + fq) ^ fsw) << 4;
+#pragma unroll
+    for (int i = 0; i < MT16; ++i) fa[slot_][i] = *reinterpret_cast<const i32x4_t*>(sa + a_off[i] + sw);
+#pragma unroll
+    for (int j = 0; j < NT16; ++j) fb[slot_][j] = *reinterpret_cast<const i32x4_t*>(sb + b_off[j] + sw);
+  };
+  i32x4_t acc[MT16][NT16];
+  auto mfmas = [&](int slot_) {
+#pragma unroll
+    for (int i = 0; i < MT16; ++i)
+#pragma unroll
+      for (int j = 0; j < NT16; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[slot_][j], fa[slot_][i], acc[i][j], 0, 0, 0);
+  };
+  // pair each fragment read of the next half with an MFMA of this one
+  auto interleave = [&]() {
+#pragma unroll
+    for (int q = 0; q < MT16 + NT16; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    if constexpr (MT16 * NT16 > MT16 + NT16)
+      __builtin_amdgcn_sched_group_barrier(0x008, MT16 * NT16 - (MT16 + NT16), 0);
+  };
+
+  setup_tile(mt, nt);
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (s < KT) issue_stage(s, s);
+  wait_groups<DPW, S - 1>(min(S - 1, KT - 1));  // step 0 landed
+  lds_barrier();
+  while (true) {
+#pragma unroll
+    for (int i = 0; i < MT16; ++i)
+#pragma unroll
+      for (int j = 0; j < NT16; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+    read_frags(0, 0, 0);
+    int buf = 0;
+    for (int kt = 0; kt < KT; ++kt) {
+      read_frags(buf, 1, 1);
+      interleave();
+      mfmas(0);
+      const int nbuf = (buf + 1 == S) ? 0 : buf + 1;
+      if (kt + 1 < KT) {
+        wait_groups<DPW, S - 2>(min(S - 2, KT - 2 - kt));
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        read_frags(nbuf, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + S < KT) issue_stage(kt + S, buf);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      mfmas(1);
+      buf = nbuf;
+    }
+
+    // ---- next tile's first stages, then this tile's epilogue ----
+    int nmt = 0, nnt = 0;
+    const int nlogical = seek(logical + walk.G, nmt, nnt);
+    const bool has_next = nlogical < walk.total;
+    const int t_e = src.e, t_row0 = src.row0, t_rows = src.rows, t_nt = kHalves ? nt >> 1 : nt;
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();  // every wave is done reading the stage buffers
+    __builtin_amdgcn_sched_barrier(0);
+    if (has_next) {
+      setup_tile(nmt, nnt);
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (s < KT) issue_stage(s, s);
+    }
+    store_sums<T, kGateUp, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, t_e, wm, wn, t_row0, t_rows, t_nt);
+    if (!has_next) break;
+    logical = nlogical;
+    mt = nmt;
+    nt = nnt;
+    wait_vmcnt<0>();  // the next tile's stages (and this wave's stores) are done
+    lds_barrier();
+  }
+}
+
+using SmallCfg = TileCfg<kMfmaSmallBM, 256, 4, 1, 4, 8>;
+using MidCfg = TileCfg<kMfmaMidBM, 256, 3, 2, 4, 8>;
+using Mid2Cfg = TileCfg<kMfmaMid2BM, 256, 3, 2, 4, 8>;
+using NarrowCfg = TileCfg<kMfmaMid2BM, 128, 4, 4, 2, 8>;
+using NarrowMidCfg = TileCfg<kMfmaMidBM, 128, 3, 2, 2, 8>;
+
+Args args_of(const Int8Gemm& g) {
+  Args a{};
+  a.a = g.a, a.a_scale = g.a_scale, a.row_src = g.row_src;
+  a.tiles = RowTiles{g.tiles, (int)g.n_rows, g.block_m};
+  a.w0 = g.w0, a.w1 = g.w1, a.s0 = g.s0, a.s1 = g.s1, a.bias = g.bias;
+  a.kp = (int)g.kp, a.n = (int)g.n, a.capacity = (int)g.capacity, a.c = g.c;
+  return a;
+}
+
+template <typename Cfg, typename T, bool kGateUp, bool kGather, bool kHalves = false>
+int launch_tiles(const Int8Gemm& g, hipStream_t s) {
+  if (g.capacity == 0) return ASTRAI_MOE_OK;
+  Args a = args_of(g);
+  const int64_t n_tiles_n = ceil_div(g.n, kGateUp ? Cfg::BN / 2 : Cfg::BN);  // the last may be partial
+  a.n_tiles_n = (int)n_tiles_n;
+  int64_t grid = 0;
+  if (int rc = persistent_grid(g.capacity, kHalves ? 2 * n_tiles_n : n_tiles_n, &grid)) return rc;
+  hipLaunchKernelGGL((gemm_i8_kernel<Cfg, T, kGateUp, kGather, kHalves>), dim3((unsigned)grid), dim3(Cfg::THREADS), 0, s,
+                     a);
+  return check_launch(kGateUp ? "gemm_i8_kernel<gate_up>" : "gemm_i8_kernel<down>");
+}
+
+template <typename T, bool kGateUp, bool kGather>
+int launch_typed(const Int8Gemm& g, hipStream_t s) {
+  const Tiles pick = pick_tiles(g.rows, g.block_m, g.kp / 2, g.n, kGateUp).tiles;
+  if (pick == Tiles::kHalves) return launch_tiles<Mid2Cfg, T, kGateUp, kGather, true>(g, s);
+  if (pick == Tiles::kNarrowMid) return launch_tiles<NarrowMidCfg, T, kGateUp, kGather>(g, s);
+  if (pick == Tiles::kNarrow) return launch_tiles<NarrowCfg, T, kGateUp, kGather>(g, s);
+  if (pick == Tiles::kNarrowHalves) return launch_tiles<NarrowCfg, T, kGateUp, kGather, true>(g, s);
+  if (g.block_m == kMfmaBigBM) return launch_tiles<Mid2Cfg, T, kGateUp, kGather, true>(g, s);
+  if (g.block_m == kMfmaMidBM) return launch_tiles<MidCfg, T, kGateUp, kGather>(g, s);
+  if (g.block_m == kMfmaMid2BM) return launch_tiles<Mid2Cfg, T, kGateUp, kGather>(g, s);
+  return launch_tiles<SmallCfg, T, kGateUp, kGather>(g, s);
+}
+
+}  // namespace
+
+#if ASTRAI_MOE_RAGGED_K
+namespace ragged {
+#endif
+
+int launch_int8_mfma(const Int8Gemm& g, hipStream_t s) {
+#if !ASTRAI_MOE_RAGGED_K
+  const int size = g.dtype == ASTRAI_MOE_BF16 ? 2 : 4;
+  if (g.kp % kRowBytes != 0 || g.n * size % 16 != 0 || g.n % 4 != 0 || !aligned16(g.c))
+    return ragged::launch_int8_mfma(g, s);
+#endif
+  // (the gate/up products gather their rows, the others take them as they lie)
+  if (g.dtype == ASTRAI_MOE_BF16)
+    return g.w1 != nullptr ? launch_typed<bf16_t, true, true>(g, s) : launch_typed<bf16_t, false, false>(g, s);
+  return g.w1 != nullptr ? launch_typed<float, true, true>(g, s) : launch_typed<float, false, false>(g, s);
+}
+
+#if ASTRAI_MOE_RAGGED_K
+}  // namespace ragged
+#endif
+
+}  // namespace astrai_moe

@@ -17,6 +17,8 @@ constexpr int64_t kInt8MaxK = 131072;
 // rounded to dtype: one product and bias, or (w1 set) silu(g) * u of the products
 // g with w0 and u with w1.
 struct Int8Gemm {
+  RowCounts rows;         // the rows as far as the host knows them
+  int64_t a_bytes = 0;    // of a, where gathered
   const int8_t* a;        // [*, kp]
   const float* a_scale;   // [*]
   const int32_t* row_src;
@@ -53,5 +55,13 @@ __device__ __forceinline__ float swiglu<bf16_t>(int g, int u, float sa, float sg
 
 int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, float* scale, hipStream_t s);
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s);
+
+// On the matrix cores (moe_gemm_int8.hip); gate/up products are gathered (row_src),
+// the others not. a under 4 GiB where gathered. ragged: rows of a partial K step, or
+// outputs whose rows are no whole number of 16 bytes.
+int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
+namespace ragged {
+int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
+}
 
 }  // namespace astrai_moe

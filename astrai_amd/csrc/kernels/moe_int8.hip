@@ -192,6 +192,18 @@ int check_int8(const char* who, int dtype, int64_t k, int64_t n) {
   return ASTRAI_MOE_OK;
 }
 
+// Row-tile heights: those of the bf16 products (astrai_moe_select_block_m), whose
+// tiles take the same time a step.
+int layer_block_m(int64_t rows_per_expert) {
+  return rows_per_expert < 24    ? kMfmaSmallBM
+         : rows_per_expert < 48  ? kMfmaMidBM
+         : rows_per_expert < 128 ? kMfmaMid2BM
+                                 : kMfmaBigBM;
+}
+int linear_block_m(int64_t n_rows, int64_t kp, int64_t n) {
+  return n_rows < 96 ? kMfmaSmallBM : dense_gemm_block_m(n_rows, kp / 2, n, false);
+}
+
 struct Parts {  // of a workspace, 256-byte aligned
   int64_t bytes = 0;
   int64_t take(int64_t n) {
@@ -243,7 +255,7 @@ struct LayerPlan {
     experts = z.n_experts + z.n_shared;
     slots = z.top_k + z.n_shared;
     rows = T * slots;
-    block_m = 64;
+    block_m = layer_block_m(T * z.top_k / z.n_experts);
     tiles_len = astrai_moe_tile_list_len(T, experts, slots, block_m);
     dp = int8_row_bytes(z.dim);
     fp = int8_row_bytes(z.dim_ffn);
@@ -282,6 +294,8 @@ int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, in
 }
 
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s) {
+  if ((g.w1 != nullptr) == (g.row_src != nullptr) && (g.row_src == nullptr || g.a_bytes < (1ll << 32)))
+    return launch_int8_mfma(g, s);
   return g.dtype == ASTRAI_MOE_BF16 ? launch_general<bf16_t>(g, s) : launch_general<float>(g, s);
 }
 
@@ -329,10 +343,10 @@ extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
   int8_t* const q = reinterpret_cast<int8_t*>(base + p.q);
   float* const scale = reinterpret_cast<float*>(base + p.scale);
   if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, scale, s)) return rc;
-  Int8Gemm g{};
+  Int8Gemm g{RowCounts(n_rows, 1)};
   g.a = q, g.a_scale = scale, g.w0 = w, g.s0 = w_scale, g.bias = bias;
   g.kp = int8_row_bytes(k), g.n = n, g.dtype = dtype, g.c = out;
-  g.n_rows = n_rows, g.block_m = 64, g.capacity = ceil_div(n_rows, g.block_m);
+  g.n_rows = n_rows, g.block_m = linear_block_m(n_rows, g.kp, n), g.capacity = ceil_div(n_rows, g.block_m);
   return launch_int8_gemm(g, s);
 }
 
@@ -380,15 +394,16 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
   else
     rc = launch_route(logits, dtype, n_tokens, n_experts, top_k, n_shared, topk_idx, base + p.topk_w, hist, s);
   if (rc) return rc;
-  if ((rc = astrai_moe_permute(topk_idx, base + p.topk_w, hist, nullptr, dtype, n_tokens, p.experts, p.slots, dim,
+  if ((rc = astrai_moe_permute(topk_idx, base + p.topk_w, hist, nullptr, dtype, n_tokens, p.experts, p.slots, p.dp / 2,
                                p.block_m, i32(p.offsets), i32(p.sorted_token), base + p.sorted_w, i32(p.token_pos),
                                nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
     return rc;
   if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq), f32(p.xs), s))) return rc;
-  Int8Gemm g{};
+  Int8Gemm g{RowCounts(n_tokens * top_k, n_experts, n_shared, n_tokens)};
   g.a = i8(p.xq), g.a_scale = f32(p.xs), g.row_src = i32(p.sorted_token);
   g.tiles = tiles, g.capacity = (p.tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE;
   g.w0 = w_gate, g.w1 = w_up, g.s0 = gate_scale, g.s1 = up_scale;
+  g.a_bytes = n_tokens * p.dp;
   g.kp = p.dp, g.n = dim_ffn, g.dtype = dtype, g.c = base + p.h, g.block_m = p.block_m;
   if ((rc = launch_int8_gemm(g, s))) return rc;
   if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq), f32(p.hs), s))) return rc;
