@@ -138,8 +138,8 @@ struct TileWalk {
         total(n_live * n_tiles_n),
         group_size(GM * n_tiles_n) {}
   // n_live_ row tiles known without a list
-  __device__ TileWalk(int n_live_, int n_tiles_n)
-      : G((int)gridDim.x), n_live(n_live_), total(n_live_ * n_tiles_n), group_size(GM * n_tiles_n) {}
+  __device__ TileWalk(int n_live_, int n_tiles_n, int G_ = 0)
+      : G(G_ > 0 ? G_ : (int)gridDim.x), n_live(n_live_), total(n_live_ * n_tiles_n), group_size(GM * n_tiles_n) {}
   __device__ int first_slot() const {
     const int bid = blockIdx.x;
     return (G % kXcds == 0) ? (bid % kXcds) * (G / kXcds) + bid / kXcds : bid;
@@ -196,11 +196,17 @@ struct SplitWalk : TileWalk<GM> {
   int full, S, KT;
   __device__ SplitWalk(const int32_t* tiles, int capacity, int n_tiles_n, int KT_, bool split, int G_ = 0)
       : TileWalk<GM>(tiles, capacity, n_tiles_n, G_), full(this->total), S(1), KT(KT_) {
-    if (split) {
-      const int L = this->total % this->G;
-      const int s = (L > 0 && 2 * L <= this->G) ? min(this->G / L, KT / kSplitMinSteps) : 1;
-      if (s >= 2) S = s, full = this->total - L;
-    }
+    if (split) split_tail();
+  }
+  // row tiles known without a list
+  __device__ SplitWalk(int n_live_, int n_tiles_n, int KT_, bool split, int G_ = 0)
+      : TileWalk<GM>(n_live_, n_tiles_n, G_), full(this->total), S(1), KT(KT_) {
+    if (split) split_tail();
+  }
+  __device__ void split_tail() {
+    const int L = this->total % this->G;
+    const int s = (L > 0 && 2 * L <= this->G) ? min(this->G / L, KT / kSplitMinSteps) : 1;
+    if (s >= 2) S = s, full = this->total - L;
   }
   __device__ int items() const { return full + (this->total - full) * S; }
   // item `i` (< items()): its tile, K steps [k0, k1) and tail unit (-1: the whole tile)

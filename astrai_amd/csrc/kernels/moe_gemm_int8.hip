@@ -171,10 +171,9 @@ __device__ __forceinline__ typename Out4<T>::type out_of(const i32x4_t& g, const
 template <typename T>
 __device__ __forceinline__ f32x4_t bias_of(const void* bias, int n, int n_all) {
   f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (bias != nullptr)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < n_all) v[r] = Elem<T>::to_f32(static_cast<const T*>(bias)[n + r]);
+  for (int r = 0; r < 4; ++r)
+    if (n + r < n_all) v[r] = Elem<T>::to_f32(static_cast<const T*>(bias)[n + r]);
   return v;
 }
 
@@ -182,7 +181,7 @@ __device__ __forceinline__ f32x4_t bias_of(const void* bias, int n, int n_all) {
 // columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile. bf16 outputs are
 // transposed in pairs of tiles to 16-byte stores; fp32 ones are 16 bytes as they
 // lie. Outputs whose rows are no whole number of 16 bytes are stored by element.
-template <typename T, bool kGateUp, int WM, int WN, int BN>
+template <typename T, bool kGateUp, bool kBias, int WM, int WN, int BN>
 __device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16], const Args& p, bool gather, int e,
                                            int wm, int wn, int t_row0, int t_rows, int t_nt) {
   constexpr int MT16 = WM / 16, NT16 = WN / 16, NJ = kGateUp ? NT16 / 2 : NT16;
@@ -193,9 +192,6 @@ __device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16
   const int N = p.n;
   T* const C = static_cast<T*>(p.c);
   const bool whole = !kRagged || (N * (int)sizeof(T)) % 16 == 0;
-  float sa[MT16];
-#pragma unroll
-  for (int i = 0; i < MT16; ++i) sa[i] = scale_of(p, gather, t_row0 + min(wm * WM + i * 16 + row_l, t_rows - 1));
 #pragma unroll
   for (int jp = 0; jp < NJ; jp += 2) {
     f32x4_t s0[2], s1[2], b[2];
@@ -204,16 +200,18 @@ __device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16
       const int n = n_base + (jp + h) * 16 + 4 * q;
       s0[h] = four(p.s0, e, n, N);
       if constexpr (kGateUp) s1[h] = four(p.s1, e, n, N);
-      b[h] = kGateUp ? f32x4_t{0, 0, 0, 0} : bias_of<T>(p.bias, n, N);
+      b[h] = kBias ? bias_of<T>(p.bias, n, N) : f32x4_t{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < MT16; ++i) {
       const int gm = wm * WM + i * 16 + row_l;
-      const int64_t row_off = (int64_t)(t_row0 + min(gm, t_rows - 1)) * N;
+      const int row = t_row0 + min(gm, t_rows - 1);
+      const float sa = scale_of(p, gather, row);
+      const int64_t row_off = (int64_t)row * N;
       typename Out4<T>::type o[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        o[h] = out_of<T, kGateUp>(acc[i][jp + h], acc[i][kGateUp ? jp + h + NJ : jp + h], sa[i], s0[h], s1[h], b[h]);
+        o[h] = out_of<T, kGateUp>(acc[i][jp + h], acc[i][kGateUp ? jp + h + NJ : jp + h], sa, s0[h], s1[h], b[h]);
       if (whole) {
         if constexpr (std::is_same_v<T, bf16_t>) {
           transpose2(o);
@@ -431,7 +429,10 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(const Args p) 
       for (int s = 0; s < S; ++s)
         if (s < KT) issue_stage(s, s);
     }
-    store_sums<T, kGateUp, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, t_e, wm, wn, t_row0, t_rows, t_nt);
+    if (!kGateUp && p.bias != nullptr)
+      store_sums<T, kGateUp, true, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, t_e, wm, wn, t_row0, t_rows, t_nt);
+    else
+      store_sums<T, kGateUp, false, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, t_e, wm, wn, t_row0, t_rows, t_nt);
     if (!has_next) break;
     logical = nlogical;
     mt = nmt;
@@ -439,6 +440,296 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(const Args p) 
     wait_vmcnt<0>();  // the next tile's stages (and this wave's stores) are done
     lds_barrier();
   }
+}
+
+// ===========================================================================
+// Streaming kernel: 256 x 256 tiles, 8 matrix-core waves + 4 DMA waves, as
+// gemm_stream_kernel of moe_gemm_mfma.hip, whose comments give the reasons of its
+// schedule: two activation and three weight stages, one barrier a K step, the
+// matrix-core waves' fragments in rings, the priority drops.
+// ===========================================================================
+template <bool kGateUp>
+struct StreamCfg {
+  static constexpr int BM = 256, BN = 256, GM = kGateUp ? 8 : 16;
+  static constexpr int WGM = 2, WGN = 4, MW = 8, DW = 4;  // matrix-core waves (WGM x WGN), DMA waves
+  static constexpr int WAVES = MW + DW, THREADS = WAVES * 64;
+  static constexpr int WM = BM / WGM, WN = BN / WGN;  // 128 x 64 per matrix-core wave
+  static constexpr int A_BYTES = BM * kRowBytes, B_BYTES = BN * kRowBytes;  // 32 KB per K step each
+  static constexpr int A_STAGES = 2, B_STAGES = 3;
+  static constexpr int A_OFF = 0, B_OFF = A_STAGES * A_BYTES;
+  static constexpr int LDS = B_OFF + B_STAGES * B_BYTES;  // 160 KB
+  static constexpr int OPS = A_BYTES / 1024 / DW;         // 1 KB DMA ops per DMA wave per operand and step
+  static constexpr int RG = 2, AR = 4, PD = 2;
+};
+
+// Position of a DMA wave in its workgroup's sequence of K steps.
+template <int BM, int BN, int GM, bool kGateUp, bool kGather>
+struct StepCursor {
+  int idx, mt, nt, kt, k1, unit;
+  bool live;
+  I8Src<BM, BN, kGateUp, kGather> src;
+  __device__ void enter(const SplitWalk<GM>& walk, int logical, const Args& p) {
+    walk.item(logical, mt, nt, kt, k1, unit);
+    src.setup(p, mt, nt);
+  }
+  __device__ void start(const SplitWalk<GM>& walk, const ItemSeq& seq, const Args& p) {
+    idx = 0, live = true;
+    enter(walk, seq.id(0), p);
+  }
+  // true when the cursor moved on to the next work item
+  __device__ bool advance(const SplitWalk<GM>& walk, const ItemSeq& seq, const Args& p) {
+    if (++kt < k1) return false;
+    const int nxt = seq.id(++idx);
+    live = nxt >= 0;
+    if (live) enter(walk, nxt, p);
+    return live;
+  }
+};
+
+template <typename T, bool kGateUp, bool kGather, bool kBias>
+__global__ __launch_bounds__(StreamCfg<kGateUp>::THREADS, 1) void gemm_i8_stream_kernel(const Args p) {
+  using Cfg = StreamCfg<kGateUp>;
+  __shared__ __attribute__((aligned(1024))) char smem[Cfg::LDS];
+  const uint32_t kp = (uint32_t)p.kp;
+  const int KT = (int)((kp + kRowBytes - 1) / kRowBytes);
+  const SplitWalk<Cfg::GM> walk(p.tiles.live(p.capacity), p.n_tiles_n, KT, !kGateUp && p.part != nullptr);
+  const ItemSeq seq(walk, KT, p.sched);
+  if (seq.m == 0) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+
+  if (wave >= Cfg::MW) {
+    // ---------------- DMA waves ----------------
+    const int dw = wave - Cfg::MW;
+    StepCursor<Cfg::BM, Cfg::BN, Cfg::GM, kGateUp, kGather> ca;  // next A step
+    StepCursor<Cfg::BM, Cfg::BN, Cfg::GM, kGateUp, false> cb;    // next B step
+    RowOffsets<Cfg::OPS, kGather> rows;
+    auto load_rows = [&]() { rows.load(p.row_src, ca.src.row0, ca.src.rows, dw * Cfg::OPS, lane, kp); };
+    ca.start(walk, seq, p);
+    cb.start(walk, seq, p);
+    load_rows();
+    auto tail_step = [&](int kt) { return kRagged && (uint32_t)(kt + 1) * kRowBytes > kp; };
+    auto ops_a = [&](auto tail_c, int buf) {
+      const DmaLane dl(lane, ca.kt);
+      char* base = smem + Cfg::A_OFF + buf * Cfg::A_BYTES;
+#pragma unroll
+      for (int i = 0; i < Cfg::OPS; ++i) {
+        const int q = dw * Cfg::OPS + i;
+        ca.src.template dma_a_rows<decltype(tail_c)::value>(dl, rows.off[i], q, kp, base + q * 1024);
+      }
+    };
+    auto issue_a = [&](int buf) {
+      if (tail_step(ca.kt))
+        ops_a(std::true_type{}, buf);
+      else
+        ops_a(std::false_type{}, buf);
+      if (ca.advance(walk, seq, p)) load_rows();  // the next item's rows
+    };
+    auto ops_b = [&](auto tail_c, int buf) {
+      const DmaLane dl(lane, cb.kt);
+      char* base = smem + Cfg::B_OFF + buf * Cfg::B_BYTES;
+#pragma unroll
+      for (int i = 0; i < Cfg::OPS; ++i) {
+        const int q = dw * Cfg::OPS + i;
+        cb.src.template dma_b<decltype(tail_c)::value>(dl, q, kp, base + q * 1024);
+      }
+    };
+    auto issue_b = [&](int buf) {
+      if (tail_step(cb.kt))
+        ops_b(std::true_type{}, buf);
+      else
+        ops_b(std::false_type{}, buf);
+      cb.advance(walk, seq, p);
+    };
+    // prologue in issue order B0, A0, B1, A1, B2 (as far as the steps exist)
+    int a_iss = 0, b_iss = 0;
+    issue_b(0), ++b_iss;
+    issue_a(0), ++a_iss;
+    if (cb.live) issue_b(1), ++b_iss;
+    if (ca.live) issue_a(1), ++a_iss;
+    if (cb.live) issue_b(2), ++b_iss;
+    wait_groups<Cfg::OPS, 3>((a_iss - 1) + (b_iss - 1));  // A0 and B0 landed
+    __builtin_amdgcn_s_barrier();                          // X_{-1}
+    for (int g = 0;; ++g) {
+      // A(g + 1) and B(g + 1) landed; B(g + 2), issued after A(g + 1), may stay in flight
+      wait_groups<Cfg::OPS, 1>(b_iss > g + 2 ? 1 : 0);
+      __builtin_amdgcn_s_barrier();  // X_g
+      const bool more = ca.live;
+      if (ca.live) issue_a(g & 1), ++a_iss;  // A(g + 2)
+      if (cb.live) issue_b(g % 3), ++b_iss;  // B(g + 3)
+      if (!more && g + 1 >= a_iss) break;    // X_g was the last step's barrier
+    }
+    return;
+  }
+
+  // ---------------- matrix-core waves ----------------
+  const int wm = wave / Cfg::WGN;
+  const int wn = wave % Cfg::WGN;
+  constexpr int MT16 = Cfg::WM / 16, NT16 = Cfg::WN / 16;
+  constexpr int AR = Cfg::AR, PD = Cfg::PD;
+  const int frag_row = lane & 15;
+  const int fq = lane >> 4;
+  const uint32_t v_lane = frag_row * kRowBytes + ((fq ^ ((frag_row >> 1) & 7)) << 4);
+  const uint32_t b_row = kGateUp ? wn * (Cfg::WN / 2) : wn * Cfg::WN;
+  uint32_t vA = (uint32_t)Cfg::A_OFF + (uint32_t)(wm * Cfg::WM) * kRowBytes + v_lane;
+  uint32_t vB = (uint32_t)Cfg::B_OFF + b_row * kRowBytes + v_lane;
+  constexpr uint32_t kBEnd = (uint32_t)Cfg::LDS;
+  auto next_b = [&](uint32_t v) -> uint32_t {
+    const uint32_t n = v + Cfg::B_BYTES;
+    return n >= kBEnd ? n - Cfg::B_STAGES * Cfg::B_BYTES : n;
+  };
+  auto rotate = [&]() {
+    vA ^= (uint32_t)Cfg::A_BYTES;
+    vB = next_b(vB);
+    asm volatile("" : "+v"(vA), "+v"(vB));
+  };
+  i32x4_t fa[AR], fb[NT16];
+  i32x4_t acc[MT16][NT16];
+  auto lds128 = [&](uint32_t addr) -> i32x4_t { return *reinterpret_cast<const i32x4_t*>(smem + addr); };
+  auto rdA = [&](uint32_t base, int kh, int i) -> i32x4_t {
+    return lds128((base ^ (kh ? 64u : 0u)) + i * 16 * kRowBytes);
+  };
+  auto rdB = [&](uint32_t base, int kh, int j) -> i32x4_t {
+    constexpr int half = NT16 / 2;
+    const int r = kGateUp ? ((j < half) ? j * 16 : Cfg::BN / 2 + (j - half) * 16) : j * 16;
+    return lds128((base ^ (kh ? 64u : 0u)) + r * kRowBytes);
+  };
+  // one K step as 16 rows of 16 (two halves x 8 row blocks) in groups of RG
+  constexpr int RG = Cfg::RG;
+  auto step = [&]() {
+    uint32_t nA = 0, nB = 0;
+    static_for<16 / RG>([&](auto gg) {
+      constexpr int r0 = decltype(gg)::value * RG;
+      if constexpr (r0 == 0) __builtin_amdgcn_s_setprio(1);
+      if constexpr (kGateUp ? (r0 == 8 || r0 == 12) : r0 == 10) __builtin_amdgcn_s_setprio(0);
+      if constexpr (kGateUp ? r0 == 10 : r0 == 12) __builtin_amdgcn_s_setprio(1);
+      if constexpr (r0 + PD >= 16 && r0 + PD < 16 + RG) {
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();  // X_g
+        __builtin_amdgcn_sched_barrier(0);
+        nA = vA ^ (uint32_t)Cfg::A_BYTES;
+        nB = next_b(vB);
+      }
+      static_for<RG>([&](auto qq) {
+        constexpr int rp = r0 + PD + decltype(qq)::value;
+        if constexpr (rp < 16)
+          fa[rp % AR] = rdA(vA, rp / 8, rp % 8);
+        else
+          fa[rp % AR] = rdA(nA, 0, rp - 16);
+      });
+#pragma unroll
+      for (int j = 0; j < NT16; ++j) {
+        static_for<RG>([&](auto qq) {
+          constexpr int r = r0 + decltype(qq)::value;
+          acc[r % 8][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j], fa[r % AR], acc[r % 8][j], 0, 0, 0);
+        });
+        if constexpr (r0 + RG == 8) fb[j] = rdB(vB, 1, j);
+        if constexpr (r0 + RG == 16) fb[j] = rdB(nB, 0, j);
+      }
+    });
+  };
+
+  lds_barrier();  // X_{-1}
+#pragma unroll
+  for (int j = 0; j < NT16; ++j) fb[j] = rdB(vB, 0, j);
+#pragma unroll
+  for (int r = 0; r < PD; ++r) fa[r % AR] = rdA(vA, 0, r);
+  int mt = 0, nt = 0, k0 = 0, k1 = 0, unit = -1;
+  bool claiming = wave == 0;  // matrix-core wave 0 makes the run-time claims
+  // Waves of padding rows only idle where gemm_stream_kernel's do.
+  const int idle_row0 = __builtin_amdgcn_readfirstlane(wm * Cfg::WM);
+  const int idle_mt0 =
+      __builtin_amdgcn_readfirstlane(KT < kIdleMaxSteps || p.tiles.tiles == nullptr ? 0 : p.tiles.tiles[3]);
+  walk.item(seq.id(0), mt, nt, k0, k1, unit);
+  for (int idx = 0;; ++idx) {
+    const int claim_at = (claiming && seq.claims_next(idx)) ? k1 - kClaimLead : -1;
+    int e, t_row0, t_end;
+    p.tiles.get(mt, e, t_row0, t_end);
+    const int t_rows = min(Cfg::BM, t_end - t_row0);
+    const bool idle = idle_threshold(mt >= idle_mt0, idle_row0) >= t_rows;
+    int zero;
+    asm("s_mov_b32 %0, 0" : "=s"(zero));
+#pragma unroll
+    for (int i = 0; i < MT16; ++i)
+#pragma unroll
+      for (int j = 0; j < NT16; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = zero;
+    if (idle) {
+      for (int kt = k0; kt < k1; ++kt) {
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();  // X_g
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + 1 == k1) {
+          const uint32_t nA = vA ^ (uint32_t)Cfg::A_BYTES, nB = next_b(vB);
+#pragma unroll
+          for (int r = 0; r < PD; ++r) fa[r % AR] = rdA(nA, 0, r);
+#pragma unroll
+          for (int j = 0; j < NT16; ++j) fb[j] = rdB(nB, 0, j);
+        }
+        rotate();
+      }
+    } else {
+      for (int kt = k0, stop = claim_at >= 0 ? claim_at : k1;; stop = k1) {
+        for (; kt < stop; ++kt) {
+          step();
+          rotate();
+        }
+        if (kt == k1) break;
+        claiming = seq.claim(idx, p.sched);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const int nxt = seq.id(idx + 1);
+    if (kGateUp || unit < 0) {
+      if (!idle)
+        store_sums<T, kGateUp, kBias, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, e, wm, wn, t_row0, t_rows, nt);
+    } else {
+      store_partial(reinterpret_cast<const f32x4_t(&)[MT16][NT16]>(acc), p.part, unit, wave, lane);
+    }
+    if (nxt < 0) break;
+    walk.item(nxt, mt, nt, k0, k1, unit);
+  }
+}
+
+// The epilogue of the split tail tiles (SplitWalk): workgroup (t, w), one wave,
+// adds the partial sums of matrix-core wave w of tail tile t.
+template <typename T, bool kBias>
+__global__ __launch_bounds__(64) void i8_split_reduce_kernel(const Args p, int G) {
+  using Cfg = StreamCfg<false>;
+  const int KT = (p.kp + kRowBytes - 1) / kRowBytes;
+  const SplitWalk<Cfg::GM> walk(p.tiles.live(p.capacity), p.n_tiles_n, KT, true, G);
+  const int t = blockIdx.x;
+  if (walk.S < 2 || t >= walk.total - walk.full) return;
+  int mt = 0, nt = 0;
+  walk.decode(walk.full + t, mt, nt);
+  int e, t_row0, t_end;
+  p.tiles.get(mt, e, t_row0, t_end);
+  const int t_rows = min(Cfg::BM, t_end - t_row0);
+  const int wave = blockIdx.y, lane = threadIdx.x;
+  constexpr int MT16 = Cfg::WM / 16, NT16 = Cfg::WN / 16;
+  constexpr int kUnitVecs = kSplitUnitFloats / 4;
+  const i32x4_t* at = reinterpret_cast<const i32x4_t*>(p.part) + (int64_t)t * walk.S * kUnitVecs +
+                      wave * (MT16 * NT16 * 64) + lane;
+  i32x4_t acc[MT16][NT16];
+#pragma unroll
+  for (int i = 0; i < MT16; ++i)
+#pragma unroll
+    for (int j = 0; j < NT16; ++j) acc[i][j] = at[(i * NT16 + j) * 64];
+  for (int s = 1; s < walk.S; ++s) {
+    const i32x4_t* ps = at + (int64_t)s * kUnitVecs;
+#pragma unroll
+    for (int i = 0; i < MT16; ++i)
+#pragma unroll
+      for (int j = 0; j < NT16; ++j) acc[i][j] += ps[(i * NT16 + j) * 64];
+  }
+  store_sums<T, false, kBias, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, false, e, wave / Cfg::WGN, wave % Cfg::WGN, t_row0,
+                                                         t_rows, nt);
+}
+
+// Clears the run-time claim counter of a streaming launch.
+__global__ __launch_bounds__(64) void i8_sched_clear_kernel(int32_t* __restrict__ sched) {
+  if (threadIdx.x == 0) sched[0] = 0;
 }
 
 using SmallCfg = TileCfg<kMfmaSmallBM, 256, 4, 1, 4, 8>;
@@ -469,6 +760,39 @@ int launch_tiles(const Int8Gemm& g, hipStream_t s) {
   return check_launch(kGateUp ? "gemm_i8_kernel<gate_up>" : "gemm_i8_kernel<down>");
 }
 
+template <typename T, bool kGateUp, bool kGather, bool kBias>
+int launch_stream(const Int8Gemm& g, hipStream_t s) {
+  if (g.capacity == 0) return ASTRAI_MOE_OK;
+  using Cfg = StreamCfg<kGateUp>;
+  Args a = args_of(g);
+  const int64_t n_tiles_n = ceil_div(g.n, kGateUp ? Cfg::BN / 2 : Cfg::BN);  // the last may be partial
+  a.n_tiles_n = (int)n_tiles_n;
+  int64_t grid = 0;
+  if (int rc = persistent_grid(g.capacity, n_tiles_n, &grid)) return rc;
+  const int64_t ksteps = ceil_div(g.kp, kRowBytes);
+  const bool have_ws = g.ws.base != nullptr && g.ws.bytes >= kSchedBytes && grid <= kMaxSchedGroups;
+  a.sched = have_ws && ksteps >= kDynamicMinSteps ? static_cast<int32_t*>(g.ws.base) : nullptr;
+  a.part = !kGateUp && have_ws && splits_tail(g.kp / 2) &&
+                   g.ws.bytes >= kSchedBytes + grid * (int64_t)sizeof(float) * kSplitUnitFloats
+               ? reinterpret_cast<float*>(static_cast<char*>(g.ws.base) + kSchedBytes)
+               : nullptr;
+  if (a.sched != nullptr) {
+    hipLaunchKernelGGL(i8_sched_clear_kernel, dim3(1), dim3(64), 0, s, a.sched);
+    if (int rc = check_launch("i8_sched_clear_kernel")) return rc;
+  }
+  hipLaunchKernelGGL((gemm_i8_stream_kernel<T, kGateUp, kGather, kBias>), dim3((unsigned)grid), dim3(Cfg::THREADS), 0,
+                     s, a);
+  if (int rc = check_launch(kGateUp ? "gemm_i8_stream_kernel<gate_up>" : "gemm_i8_stream_kernel<down>")) return rc;
+  if constexpr (!kGateUp) {
+    if (a.part == nullptr) return ASTRAI_MOE_OK;
+    // whether the tail was split is decided on the device: at most G / 2 tail tiles
+    hipLaunchKernelGGL((i8_split_reduce_kernel<T, kBias>), dim3((unsigned)((grid + 1) / 2), Cfg::MW), dim3(64), 0, s, a,
+                       (int)grid);
+    return check_launch("i8_split_reduce_kernel");
+  }
+  return ASTRAI_MOE_OK;
+}
+
 template <typename T, bool kGateUp, bool kGather>
 int launch_typed(const Int8Gemm& g, hipStream_t s) {
   const Tiles pick = pick_tiles(g.rows, g.block_m, g.kp / 2, g.n, kGateUp).tiles;
@@ -476,7 +800,14 @@ int launch_typed(const Int8Gemm& g, hipStream_t s) {
   if (pick == Tiles::kNarrowMid) return launch_tiles<NarrowMidCfg, T, kGateUp, kGather>(g, s);
   if (pick == Tiles::kNarrow) return launch_tiles<NarrowCfg, T, kGateUp, kGather>(g, s);
   if (pick == Tiles::kNarrowHalves) return launch_tiles<NarrowCfg, T, kGateUp, kGather, true>(g, s);
-  if (g.block_m == kMfmaBigBM) return launch_tiles<Mid2Cfg, T, kGateUp, kGather, true>(g, s);
+  if (g.block_m == kMfmaBigBM) {
+    // (an fp32 h, taken in 64 bits, does not fit the streaming kernel's registers)
+    if constexpr (kGateUp && std::is_same_v<T, float>)
+      return launch_tiles<Mid2Cfg, T, kGateUp, kGather, true>(g, s);
+    else if constexpr (!kGateUp)
+      if (g.bias != nullptr) return launch_stream<T, kGateUp, kGather, true>(g, s);
+    if constexpr (!(kGateUp && std::is_same_v<T, float>)) return launch_stream<T, kGateUp, kGather, false>(g, s);
+  }
   if (g.block_m == kMfmaMidBM) return launch_tiles<MidCfg, T, kGateUp, kGather>(g, s);
   if (g.block_m == kMfmaMid2BM) return launch_tiles<Mid2Cfg, T, kGateUp, kGather>(g, s);
   return launch_tiles<SmallCfg, T, kGateUp, kGather>(g, s);

@@ -32,6 +32,7 @@ struct Int8Gemm {
   void* c;                // [*, n] dtype
   int64_t n_rows;
   int block_m;
+  GemmWorkspace ws;       // of the 256-row tiles, as the bf16 products'
 };
 
 // silu(g) u of the sums of two products. An fp32 h is taken in 64 bits and rounded

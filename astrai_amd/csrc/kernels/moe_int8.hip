@@ -214,11 +214,17 @@ struct Parts {  // of a workspace, 256-byte aligned
 };
 
 struct LinearPlan {
-  int64_t q, scale, bytes;
-  LinearPlan(int64_t m, int64_t k) {
+  int block_m;
+  int64_t q, scale, gemm_ws, gemm_ws_bytes = 0, bytes;
+  LinearPlan(int64_t m, int64_t k, int64_t n) {
+    const int64_t kp = int8_row_bytes(k);
+    block_m = linear_block_m(m, kp, n);
+    if (block_m == kMfmaBigBM)
+      gemm_ws_bytes = gemm_workspace_bytes(down_splits(RowCounts(m, 1), block_m, kp / 2, n, false));
     Parts p;
-    q = p.take(m * int8_row_bytes(k));
+    q = p.take(m * kp);
     scale = p.take(m * 4);
+    gemm_ws = p.take(gemm_ws_bytes);
     bytes = p.bytes;
   }
 };
@@ -245,11 +251,13 @@ int check_layer(const LayerSizes& z) {
   return ASTRAI_MOE_OK;
 }
 
+RowCounts row_counts(const LayerSizes& z) { return {z.n_tokens * z.top_k, z.n_experts, z.n_shared, z.n_tokens}; }
+
 struct LayerPlan {
   int experts, slots, block_m;
   int64_t rows, tiles_len, dp, fp;
   int64_t topk_idx, topk_w, chunk_hist, chunk_base, offsets, sorted_token, sorted_w, token_pos, tiles, xq, xs, h, hq, hs,
-      y, bytes;
+      y, gemm_ws, gemm_ws_bytes = 0, bytes;
   explicit LayerPlan(const LayerSizes& z) {
     const int64_t size = z.dtype == ASTRAI_MOE_BF16 ? 2 : 4, T = z.n_tokens;
     experts = z.n_experts + z.n_shared;
@@ -275,6 +283,9 @@ struct LayerPlan {
     h = y = p.take(rows * std::max(z.dim_ffn, z.dim) * size);
     hq = p.take(rows * fp);
     hs = p.take(rows * 4);
+    if (block_m == kMfmaBigBM)
+      gemm_ws_bytes = gemm_workspace_bytes(down_splits(row_counts(z), block_m, fp / 2, z.dim, false));
+    gemm_ws = p.take(gemm_ws_bytes);
     bytes = p.bytes;
   }
 };
@@ -322,7 +333,7 @@ extern "C" int64_t astrai_moe_int8_linear_workspace_bytes(int64_t n_rows, int64_
   clear_error();
   if (int rc = check_int8("int8_linear", dtype, k, n)) return rc;
   ASTRAI_REQUIRE(n_rows >= 0 && n_rows < (1ll << 31), "int8_linear: n_rows must be in [0, 2^31)");
-  return LinearPlan(n_rows, k).bytes;
+  return LinearPlan(n_rows, k, n).bytes;
 }
 
 extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w, const float* w_scale,
@@ -335,7 +346,7 @@ extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
   ASTRAI_REQUIRE(x && w && w_scale && workspace && out, "int8_linear: null buffer");
   ASTRAI_REQUIRE(on16(w), "int8_linear: the weight must start on a 16-byte boundary");
   ASTRAI_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "int8_linear: workspace must be 256-byte aligned");
-  const LinearPlan p(n_rows, k);
+  const LinearPlan p(n_rows, k, n);
   ASTRAI_REQUIRE(workspace_bytes >= p.bytes, "int8_linear: workspace holds %lld bytes, needs %lld",
                  (long long)workspace_bytes, (long long)p.bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -346,7 +357,8 @@ extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
   Int8Gemm g{RowCounts(n_rows, 1)};
   g.a = q, g.a_scale = scale, g.w0 = w, g.s0 = w_scale, g.bias = bias;
   g.kp = int8_row_bytes(k), g.n = n, g.dtype = dtype, g.c = out;
-  g.n_rows = n_rows, g.block_m = linear_block_m(n_rows, g.kp, n), g.capacity = ceil_div(n_rows, g.block_m);
+  g.n_rows = n_rows, g.block_m = p.block_m, g.capacity = ceil_div(n_rows, g.block_m);
+  if (p.gemm_ws_bytes > 0) g.ws = {base + p.gemm_ws, p.gemm_ws_bytes};
   return launch_int8_gemm(g, s);
 }
 
@@ -399,7 +411,8 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
                                nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
     return rc;
   if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq), f32(p.xs), s))) return rc;
-  Int8Gemm g{RowCounts(n_tokens * top_k, n_experts, n_shared, n_tokens)};
+  Int8Gemm g{row_counts(z)};
+  if (p.gemm_ws_bytes > 0) g.ws = {base + p.gemm_ws, p.gemm_ws_bytes};
   g.a = i8(p.xq), g.a_scale = f32(p.xs), g.row_src = i32(p.sorted_token);
   g.tiles = tiles, g.capacity = (p.tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE;
   g.w0 = w_gate, g.w1 = w_up, g.s0 = gate_scale, g.s1 = up_scale;
