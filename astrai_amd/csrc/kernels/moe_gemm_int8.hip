@@ -123,10 +123,6 @@ struct RowOffsets {
   }
 };
 
-__device__ __forceinline__ float scale_of(const Args& p, bool gather, int row) {
-  return p.a_scale[gather ? p.row_src[row] : row];
-}
-
 // The scales of four columns of expert e from column n on; columns past the
 // matrix get 0.
 __device__ __forceinline__ f32x4_t four(const float* s, int64_t e, int n, int n_all) {
@@ -182,8 +178,8 @@ __device__ __forceinline__ f32x4_t bias_of(const void* bias, int n, int n_all) {
 // transposed in pairs of tiles to 16-byte stores; fp32 ones are 16 bytes as they
 // lie. Outputs whose rows are no whole number of 16 bytes are stored by element.
 template <typename T, bool kGateUp, bool kBias, int WM, int WN, int BN>
-__device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16], const Args& p, bool gather, int e,
-                                           int wm, int wn, int t_row0, int t_rows, int t_nt) {
+__device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16], const Args& p, int e, int wm, int wn,
+                                           int t_row0, int t_rows, int t_nt) {
   constexpr int MT16 = WM / 16, NT16 = WN / 16, NJ = kGateUp ? NT16 / 2 : NT16;
   static_assert(NJ % 2 == 0, "tiles are stored in pairs");
   const int el = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
@@ -206,7 +202,7 @@ __device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16
     for (int i = 0; i < MT16; ++i) {
       const int gm = wm * WM + i * 16 + row_l;
       const int row = t_row0 + min(gm, t_rows - 1);
-      const float sa = scale_of(p, gather, row);
+      const float sa = p.a_scale[row];
       const int64_t row_off = (int64_t)row * N;
       typename Out4<T>::type o[2];
 #pragma unroll
@@ -430,9 +426,9 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(const Args p) 
         if (s < KT) issue_stage(s, s);
     }
     if (!kGateUp && p.bias != nullptr)
-      store_sums<T, kGateUp, true, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, t_e, wm, wn, t_row0, t_rows, t_nt);
+      store_sums<T, kGateUp, true, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, t_e, wm, wn, t_row0, t_rows, t_nt);
     else
-      store_sums<T, kGateUp, false, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, t_e, wm, wn, t_row0, t_rows, t_nt);
+      store_sums<T, kGateUp, false, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, t_e, wm, wn, t_row0, t_rows, t_nt);
     if (!has_next) break;
     logical = nlogical;
     mt = nmt;
@@ -630,10 +626,6 @@ __global__ __launch_bounds__(StreamCfg<kGateUp>::THREADS, 1) void gemm_i8_stream
   };
 
   lds_barrier();  // X_{-1}
-#pragma unroll
-  for (int j = 0; j < NT16; ++j) fb[j] = rdB(vB, 0, j);
-#pragma unroll
-  for (int r = 0; r < PD; ++r) fa[r % AR] = rdA(vA, 0, r);
   int mt = 0, nt = 0, k0 = 0, k1 = 0, unit = -1;
   bool claiming = wave == 0;  // matrix-core wave 0 makes the run-time claims
   // Waves of padding rows only idle where gemm_stream_kernel's do.
@@ -647,6 +639,12 @@ __global__ __launch_bounds__(StreamCfg<kGateUp>::THREADS, 1) void gemm_i8_stream
     p.tiles.get(mt, e, t_row0, t_end);
     const int t_rows = min(Cfg::BM, t_end - t_row0);
     const bool idle = idle_threshold(mt >= idle_mt0, idle_row0) >= t_rows;
+    // The item's first fragments. (The step before has read them already; read again,
+    // their registers are the epilogue's in between, which spilled without.)
+#pragma unroll
+    for (int j = 0; j < NT16; ++j) fb[j] = rdB(vB, 0, j);
+#pragma unroll
+    for (int r = 0; r < PD; ++r) fa[r % AR] = rdA(vA, 0, r);
     int zero;
     asm("s_mov_b32 %0, 0" : "=s"(zero));
 #pragma unroll
@@ -660,13 +658,6 @@ __global__ __launch_bounds__(StreamCfg<kGateUp>::THREADS, 1) void gemm_i8_stream
         __builtin_amdgcn_sched_barrier(0);
         lds_barrier();  // X_g
         __builtin_amdgcn_sched_barrier(0);
-        if (kt + 1 == k1) {
-          const uint32_t nA = vA ^ (uint32_t)Cfg::A_BYTES, nB = next_b(vB);
-#pragma unroll
-          for (int r = 0; r < PD; ++r) fa[r % AR] = rdA(nA, 0, r);
-#pragma unroll
-          for (int j = 0; j < NT16; ++j) fb[j] = rdB(nB, 0, j);
-        }
         rotate();
       }
     } else {
@@ -683,7 +674,7 @@ __global__ __launch_bounds__(StreamCfg<kGateUp>::THREADS, 1) void gemm_i8_stream
     const int nxt = seq.id(idx + 1);
     if (kGateUp || unit < 0) {
       if (!idle)
-        store_sums<T, kGateUp, kBias, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, kGather, e, wm, wn, t_row0, t_rows, nt);
+        store_sums<T, kGateUp, kBias, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, e, wm, wn, t_row0, t_rows, nt);
     } else {
       store_partial(reinterpret_cast<const f32x4_t(&)[MT16][NT16]>(acc), p.part, unit, wave, lane);
     }
@@ -723,7 +714,7 @@ __global__ __launch_bounds__(64) void i8_split_reduce_kernel(const Args p, int G
 #pragma unroll
       for (int j = 0; j < NT16; ++j) acc[i][j] += ps[(i * NT16 + j) * 64];
   }
-  store_sums<T, false, kBias, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, false, e, wave / Cfg::WGN, wave % Cfg::WGN, t_row0,
+  store_sums<T, false, kBias, Cfg::WM, Cfg::WN, Cfg::BN>(acc, p, e, wave / Cfg::WGN, wave % Cfg::WGN, t_row0,
                                                          t_rows, nt);
 }
 

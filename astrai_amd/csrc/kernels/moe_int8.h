@@ -12,15 +12,15 @@ inline int64_t int8_row_bytes(int64_t k) { return ceil_div(k, 16) * 16; }
 // Longest row whose products of codes, at most 127 * 128 each, add up below 2^31.
 constexpr int64_t kInt8MaxK = 131072;
 
-// C[r, n] = a_scale[src] w_scale[e, n] sum_k a[src, k] w[e, n, k] over the rows r of
-// the tile list (src = row_src[r], or r without row_src; e = the tile's expert),
+// C[r, n] = a_scale[r] w_scale[e, n] sum_k a[src, k] w[e, n, k] over the rows r of the
+// tile list (src = row_src[r], or r without row_src; e = the tile's expert),
 // rounded to dtype: one product and bias, or (w1 set) silu(g) * u of the products
 // g with w0 and u with w1.
 struct Int8Gemm {
   RowCounts rows;         // the rows as far as the host knows them
   int64_t a_bytes = 0;    // of a, where gathered
   const int8_t* a;        // [*, kp]
-  const float* a_scale;   // [*]
+  const float* a_scale;   // by row r
   const int32_t* row_src;
   const int32_t* tiles;   // null: one expert's n_rows rows, in tiles of block_m
   int64_t capacity;       // tiles the list holds (without a list: ceil(n_rows / block_m))
@@ -54,7 +54,6 @@ __device__ __forceinline__ float swiglu<bf16_t>(int g, int u, float sa, float sg
   return gf * __builtin_amdgcn_rcpf(1.0f + ex) * ((float)u * (sa * su));
 }
 
-int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, float* scale, hipStream_t s);
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s);
 
 // On the matrix cores (moe_gemm_int8.hip); gate/up products are gathered (row_src),

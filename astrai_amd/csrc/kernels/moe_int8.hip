@@ -18,42 +18,186 @@
 namespace astrai_moe {
 namespace {
 
-// round-half-even of 127 x / max: in 64 bits 127 x is exact, and a quotient of two
-// 32-bit values cannot round onto a half it is not equal to.
-__device__ __forceinline__ int code_of(float x, double most) { return (int)rint((double)x * 127.0 / most); }
+// round-half-even of 127 x / most, |x| <= most, exactly: n = the nearest integer to
+// the product with a rounded reciprocal is off by one at most, and the remainder 127
+// x - n most decides. C holds it exactly: 127 x and n most have 7 more bits than x
+// and most, and where n is not 0 their exponents are within 8 of each other (bf16
+// in 32 bits, fp32 in 64).
+template <typename C>
+__device__ __forceinline__ int code_of(C x, C most, C inv) {
+  C n = __builtin_elementwise_rint(x * inv);
+  const C d = __builtin_elementwise_fma(-n, most, x * (C)127), twice = (C)2 * __builtin_elementwise_abs(d);
+  const int i = (int)n;
+  const bool away = twice > most || (twice == most && (i & 1) != 0);
+  return away ? i + (d > (C)0 ? 1 : -1) : i;
+}
 
-// One wave per row: its maximum, then its codes, 16 at a time with the zeros
-// behind column k.
 template <typename T>
+struct CodeType {
+  typedef float type;  // of bf16
+};
+template <>
+struct CodeType<float> {
+  typedef double type;
+};
+
+// A power of two that brings a row's maximum away from the ends of the range, where
+// 127 x or 127 / most would leave it. (Values that vanish by it have code 0.)
+__device__ __forceinline__ float range_shift(float most) {
+  return most >= 0x1p100f ? 0x1p-64f : most < 0x1p-60f ? 0x1p64f : 1.0f;
+}
+
+// Where a row's scale goes: scale[r], or the places of its token's rows in the
+// permuted order.
+struct ScaleOut {
+  float* scale;
+  const int32_t* token_pos;  // [n_rows, slots], or null
+  int slots;
+  __device__ void put(int64_t r, float v, int lane) const {
+    if (token_pos == nullptr) {
+      if (lane == 0) scale[r] = v;
+    } else if (lane < slots) {
+      scale[token_pos[r * slots + lane]] = v;
+    }
+  }
+};
+
+// One row per WAVES waves, held in registers between its maximum and its codes: a
+// thread has NV units of 8 columns, WAVES * 512 columns apart. kVec: rows start on
+// 16-byte boundaries. One read of x and one write of the codes, bound by these: 117 M
+// values of 8192 rows 100 us, 32768 rows of 14336 XX us (XX TB/s).
+template <typename T, int WAVES, int NV, bool kVec>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
-                                                            int64_t kp, int8_t* __restrict__ q,
-                                                            float* __restrict__ scale) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (r >= n_rows) return;
-  const T* const row = x + r * k;
+                                                            int64_t kp, int8_t* __restrict__ q, const ScaleOut out) {
+  using C = typename CodeType<T>::type;
+  constexpr int ROWS = 4 / WAVES;
+  __shared__ float s_most[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * ROWS + (WAVES == 1 ? wave : 0);
+  const bool on = r < n_rows;
+  const T* const row = x + (on ? r : 0) * k;
+  const int c0 = (WAVES == 1 ? lane : (int)threadIdx.x) * 8;
+  float v[NV][8];
   float most = 0.0f;
-  bool bad = false;
-  for (int64_t c = lane; c < k; c += 64) {
-    const float v = fabsf(Elem<T>::to_f32(row[c]));
-    bad |= !(v < INFINITY);
-    most = fmaxf(most, v);
-  }
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-  bad = __any(bad);
-  if (lane == 0) scale[r] = bad ? NAN : most / 127.0f;
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * WAVES * 512;
+    if (kVec && c + 8 <= k && on) {
+      alignas(16) T in[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += 16 / (int)sizeof(T))
+        *reinterpret_cast<uint4*>(in + j) = *reinterpret_cast<const uint4*>(row + c + j);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = Elem<T>::to_f32(in[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = c + j < k && on ? Elem<T>::to_f32(row[c + j]) : 0.0f;
+    }
+  }
+  // (as integers, which order the magnitudes of floats, NaN above infinity)
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  if constexpr (WAVES > 1) {
+    if (lane == 0) s_most[wave] = __uint_as_float(top);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = max(top, __float_as_uint(s_most[w]));
+  }
+  if (!on) return;
+  most = __uint_as_float(top);
+  const bool bad = top >= 0x7f800000u;
+  if (WAVES == 1 || wave == 0) out.put(r, bad ? NAN : most / 127.0f, lane);
+  const float shift = range_shift(most);
+  const C m = (C)most * (C)shift, inv = (C)127 / m;
   const bool zero = bad || most == 0.0f;
-  for (int64_t c0 = lane * 16; c0 < kp; c0 += 64 * 16) {
-    union {
-      int8_t b[16];
-      uint4 v;
-    } out;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      out.b[j] = !zero && c0 + j < k ? (int8_t)code_of(Elem<T>::to_f32(row[c0 + j]), (double)most) : (int8_t)0;
-    *reinterpret_cast<uint4*>(q + r * kp + c0) = out.v;
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * WAVES * 512;
+    if (c >= kp) continue;
+    union {
+      int8_t b[8];
+      uint2 u;
+    } o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o.b[j] = zero ? (int8_t)0 : (int8_t)code_of<C>((C)v[i][j] * (C)shift, m, inv);
+    *reinterpret_cast<uint2*>(q + r * kp + c) = o.u;
   }
+}
+
+// Rows longer than the registers of a workgroup: read twice.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
+                                                                 int64_t kp, int8_t* __restrict__ q,
+                                                                 const ScaleOut out) {
+  using C = typename CodeType<T>::type;
+  __shared__ uint32_t s_top[4];
+  const int64_t r = blockIdx.x;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const T* const row = x + r * k;
+  uint32_t top = 0;
+  for (int64_t c = threadIdx.x; c < k; c += 256) top = max(top, __float_as_uint(Elem<T>::to_f32(row[c])) & 0x7fffffffu);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  if (lane == 0) s_top[wave] = top;
+  __syncthreads();
+  top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+  const float most = __uint_as_float(top);
+  const bool bad = top >= 0x7f800000u, zero = bad || most == 0.0f;
+  if (wave == 0) out.put(r, bad ? NAN : most / 127.0f, lane);
+  const float shift = range_shift(most);
+  const C m = (C)most * (C)shift, inv = (C)127 / m;
+  for (int64_t c0 = threadIdx.x * 8; c0 < kp; c0 += 256 * 8) {
+    union {
+      int8_t b[8];
+      uint2 u;
+    } o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      o.b[j] = zero || c0 + j >= k ? (int8_t)0 : (int8_t)code_of<C>((C)Elem<T>::to_f32(row[c0 + j]) * (C)shift, m, inv);
+    *reinterpret_cast<uint2*>(q + r * kp + c0) = o.u;
+  }
+}
+
+template <typename T, int WAVES, int NV>
+void launch_quantize_cfg(const void* x, bool vec, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out,
+                         hipStream_t s) {
+  hipLaunchKernelGGL((vec ? quantize_rows_kernel<T, WAVES, NV, true> : quantize_rows_kernel<T, WAVES, NV, false>),
+                     dim3((unsigned)ceil_div(n_rows, 4 / WAVES)), dim3(256), 0, s, static_cast<const T*>(x), n_rows, k,
+                     int8_row_bytes(k), q, out);
+}
+
+// A wave per row up to 1024 columns, a workgroup beyond.
+template <typename T>
+int launch_quantize(const void* x, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out, hipStream_t s) {
+  const bool vec = k * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  if (k <= 512)
+    launch_quantize_cfg<T, 1, 1>(x, vec, n_rows, k, q, out, s);
+  else if (k <= 1024)
+    launch_quantize_cfg<T, 1, 2>(x, vec, n_rows, k, q, out, s);
+  else if (k <= 2048)
+    launch_quantize_cfg<T, 4, 1>(x, vec, n_rows, k, q, out, s);
+  else if (k <= 4096)
+    launch_quantize_cfg<T, 4, 2>(x, vec, n_rows, k, q, out, s);
+  else if (k <= 8192)
+    launch_quantize_cfg<T, 4, 4>(x, vec, n_rows, k, q, out, s);
+  else if (k <= 16384)
+    launch_quantize_cfg<T, 4, 8>(x, vec, n_rows, k, q, out, s);
+  else
+    hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3((unsigned)n_rows), dim3(256), 0, s,
+                       static_cast<const T*>(x), n_rows, k, int8_row_bytes(k), q, out);
+  return check_launch("quantize_rows_kernel");
+}
+
+int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out,
+                         hipStream_t s) {
+  if (n_rows == 0) return ASTRAI_MOE_OK;
+  return dtype == ASTRAI_MOE_BF16 ? launch_quantize<bf16_t>(x, n_rows, k, q, out, s)
+                                  : launch_quantize<float>(x, n_rows, k, q, out, s);
 }
 
 // The product for every shape: 64 x 64 tiles, 64 bytes of K staged at a time, four
@@ -123,7 +267,7 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
       const int64_t in = rs + ty + 16 * i;
       if (in >= rows) continue;
       const int64_t row = row0 + in;
-      const float sa = p.a_scale[p.row_src != nullptr ? p.row_src[row] : row];
+      const float sa = p.a_scale[row];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t n = n0 + tx + 16 * j;
@@ -155,33 +299,61 @@ int launch_general(const Int8Gemm& g, hipStream_t s) {
 // out[t] = sum over the routed slots of w y + (sum over the shared ones of y) /
 // n_shared: 32-bit sums in the order of the slots, rounded once. A slot of weight 0
 // adds nothing, whatever its row holds (padding tokens have only such).
-template <typename T>
+// One workgroup per token (and 2048 columns), a thread per VW columns; the rows' loads
+// of up to 8 slots in flight at a time.
+template <typename T, int VW>
 __global__ __launch_bounds__(256) void sum_slots_kernel(const T* __restrict__ y, const int32_t* __restrict__ token_pos,
                                                         const T* __restrict__ topk_w, int64_t n_tokens, int top_k,
                                                         int n_shared, int64_t dim, T* __restrict__ out) {
+  struct alignas(VW * sizeof(T)) Vec {
+    T v[VW];
+  };
   const int64_t t = blockIdx.x;
   const int slots = top_k + n_shared;
   const float part = n_shared > 0 ? 1.0f / (float)n_shared : 0.0f;
-  for (int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x; c < dim; c += (int64_t)gridDim.y * 256) {
-    float sum = 0.0f;
-    for (int k = 0; k < slots; ++k) {
-      const float w = k < top_k ? Elem<T>::to_f32(topk_w[t * slots + k]) : part;
-      if (w != 0.0f) sum += w * Elem<T>::to_f32(y[(int64_t)token_pos[t * slots + k] * dim + c]);
+  for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * VW; c < dim; c += (int64_t)gridDim.y * 256 * VW) {
+    float sum[VW] = {};
+    for (int k0 = 0; k0 < slots; k0 += 8) {
+      Vec in[8];
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = 0.0f;
+        if (k0 + j < slots) {
+          w[j] = k0 + j < top_k ? Elem<T>::to_f32(topk_w[t * slots + k0 + j]) : part;
+          in[j] = *reinterpret_cast<const Vec*>(y + (int64_t)token_pos[t * slots + k0 + j] * dim + c);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (w[j] != 0.0f)
+#pragma unroll
+          for (int i = 0; i < VW; ++i) sum[i] = fmaf(w[j], Elem<T>::to_f32(in[j].v[i]), sum[i]);
     }
-    out[t * dim + c] = Elem<T>::from_f32(sum);
+    Vec o;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) o.v[i] = Elem<T>::from_f32(sum[i]);
+    *reinterpret_cast<Vec*>(out + t * dim + c) = o;
   }
+}
+
+template <typename T>
+int launch_sum_typed(const void* y, const int32_t* token_pos, const void* topk_w, int64_t n_tokens, int top_k,
+                     int n_shared, int64_t dim, void* out, hipStream_t s) {
+  constexpr int kVW = 16 / sizeof(T);
+  const bool vec = dim % kVW == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;  // (y is the workspace's)
+  const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>(ceil_div(dim, 256 * (vec ? kVW : 1)), 64));
+  hipLaunchKernelGGL((vec ? sum_slots_kernel<T, kVW> : sum_slots_kernel<T, 1>), grid, dim3(256), 0, s,
+                     static_cast<const T*>(y), token_pos, static_cast<const T*>(topk_w), n_tokens, top_k, n_shared, dim,
+                     static_cast<T*>(out));
+  return check_launch("sum_slots_kernel");
 }
 
 int launch_sum_slots(const void* y, const int32_t* token_pos, const void* topk_w, int dtype, int64_t n_tokens,
                      int top_k, int n_shared, int64_t dim, void* out, hipStream_t s) {
-  const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>(ceil_div(dim, 256), 64));
-  if (dtype == ASTRAI_MOE_BF16)
-    hipLaunchKernelGGL(sum_slots_kernel<bf16_t>, grid, dim3(256), 0, s, static_cast<const bf16_t*>(y), token_pos,
-                       static_cast<const bf16_t*>(topk_w), n_tokens, top_k, n_shared, dim, static_cast<bf16_t*>(out));
-  else
-    hipLaunchKernelGGL(sum_slots_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(y), token_pos,
-                       static_cast<const float*>(topk_w), n_tokens, top_k, n_shared, dim, static_cast<float*>(out));
-  return check_launch("sum_slots_kernel");
+  return dtype == ASTRAI_MOE_BF16
+             ? launch_sum_typed<bf16_t>(y, token_pos, topk_w, n_tokens, top_k, n_shared, dim, out, s)
+             : launch_sum_typed<float>(y, token_pos, topk_w, n_tokens, top_k, n_shared, dim, out, s);
 }
 
 int check_int8(const char* who, int dtype, int64_t k, int64_t n) {
@@ -278,7 +450,7 @@ struct LayerPlan {
     token_pos = p.take(rows * 4);
     tiles = p.take(tiles_len * 4);
     xq = p.take(T * dp);
-    xs = p.take(T * 4);
+    xs = p.take(rows * 4);  // by permuted row
     // h is read once, to be quantised, before the down product writes y
     h = y = p.take(rows * std::max(z.dim_ffn, z.dim) * size);
     hq = p.take(rows * fp);
@@ -291,18 +463,6 @@ struct LayerPlan {
 };
 
 }  // namespace
-
-int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, float* scale, hipStream_t s) {
-  if (n_rows == 0) return ASTRAI_MOE_OK;
-  const int64_t grid = ceil_div(n_rows, 4), kp = int8_row_bytes(k);
-  if (dtype == ASTRAI_MOE_BF16)
-    hipLaunchKernelGGL(quantize_rows_kernel<bf16_t>, dim3((unsigned)grid), dim3(256), 0, s,
-                       static_cast<const bf16_t*>(x), n_rows, k, kp, q, scale);
-  else
-    hipLaunchKernelGGL(quantize_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s,
-                       static_cast<const float*>(x), n_rows, k, kp, q, scale);
-  return check_launch("quantize_rows_kernel");
-}
 
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s) {
   if ((g.w1 != nullptr) == (g.row_src != nullptr) && (g.row_src == nullptr || g.a_bytes < (1ll << 32)))
@@ -326,7 +486,7 @@ extern "C" int astrai_moe_quantize_rows(const void* x, int dtype, int64_t n_rows
   if (n_rows == 0) return ASTRAI_MOE_OK;
   ASTRAI_REQUIRE(x && q && scale, "quantize_rows: null buffer");
   ASTRAI_REQUIRE(on16(q), "quantize_rows: q must start on a 16-byte boundary");
-  return launch_quantize_rows(x, dtype, n_rows, k, q, scale, static_cast<hipStream_t>(stream));
+  return launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t astrai_moe_int8_linear_workspace_bytes(int64_t n_rows, int64_t k, int64_t n, int dtype) {
@@ -353,7 +513,7 @@ extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
   char* const base = static_cast<char*>(workspace);
   int8_t* const q = reinterpret_cast<int8_t*>(base + p.q);
   float* const scale = reinterpret_cast<float*>(base + p.scale);
-  if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, scale, s)) return rc;
+  if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, s)) return rc;
   Int8Gemm g{RowCounts(n_rows, 1)};
   g.a = q, g.a_scale = scale, g.w0 = w, g.s0 = w_scale, g.bias = bias;
   g.kp = int8_row_bytes(k), g.n = n, g.dtype = dtype, g.c = out;
@@ -410,7 +570,8 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
                                p.block_m, i32(p.offsets), i32(p.sorted_token), base + p.sorted_w, i32(p.token_pos),
                                nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
     return rc;
-  if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq), f32(p.xs), s))) return rc;
+  if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq),
+                                 ScaleOut{f32(p.xs), i32(p.token_pos), p.slots}, s))) return rc;
   Int8Gemm g{row_counts(z)};
   if (p.gemm_ws_bytes > 0) g.ws = {base + p.gemm_ws, p.gemm_ws_bytes};
   g.a = i8(p.xq), g.a_scale = f32(p.xs), g.row_src = i32(p.sorted_token);
@@ -419,7 +580,8 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
   g.a_bytes = n_tokens * p.dp;
   g.kp = p.dp, g.n = dim_ffn, g.dtype = dtype, g.c = base + p.h, g.block_m = p.block_m;
   if ((rc = launch_int8_gemm(g, s))) return rc;
-  if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq), f32(p.hs), s))) return rc;
+  if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq),
+                                 ScaleOut{f32(p.hs), nullptr, 0}, s))) return rc;
   g.a = i8(p.hq), g.a_scale = f32(p.hs), g.row_src = nullptr;
   g.w0 = w_down, g.w1 = nullptr, g.s0 = down_scale, g.s1 = nullptr;
   g.kp = p.fp, g.n = dim, g.c = base + p.y;
