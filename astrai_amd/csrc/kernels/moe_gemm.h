@@ -290,7 +290,7 @@ int launch_route_scores(const void* logits, int dtype, const float* bias,
                         int weight_dtype, int32_t* topk_idx, void* topk_w,
                         int32_t* chunk_hist, hipStream_t s);
 
-// launch_route for at most ASTRAI_MOE_CHUNK_TOKENS tokens, straight to what
+// Both for at most ASTRAI_MOE_CHUNK_TOKENS tokens, straight to what
 // astrai_moe_permute writes of the decisions (tiles of block_m >= 32 rows, so one
 // for every expert that has any); neither x_perm nor expert offsets.
 struct RouteList {
@@ -304,6 +304,11 @@ struct RouteList {
 int launch_route_list(const void* logits, int dtype, int64_t n_tokens,
                       int n_experts, int top_k, int n_shared,
                       const RouteList& list, hipStream_t s);
+int launch_route_scores_list(const void* logits, int dtype, const float* bias,
+                             const astrai_moe_routing& opt, int64_t n_tokens,
+                             int n_experts, int top_k, int n_shared,
+                             int weight_dtype, const RouteList& list,
+                             hipStream_t s);
 
 // astrai_moe_combine with token_pos rows pos_stride >= top_k wide, of which
 // the first top_k are combined (moe_combine.hip).
