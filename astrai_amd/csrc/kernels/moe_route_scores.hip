@@ -17,16 +17,17 @@
 // NaN turns its expert off.
 //
 // The choice is that of exact scores as far as 64 bits tell them apart. Without a
-// bias it goes by the logits, of which every score is a rising function. With one it
-// is made in 32 bits, and again in 64 where two neighbours of the order, or the two
-// groups at the border, are closer than the scores' errors in 32 (kTol), or a row
-// holds what is no number or too few live experts (choose_slowly).
+// bias it goes by the logits, of which every score is a rising function. With one, and
+// for groups valued by two scores, it is made in 32 bits, and again in 64 where two
+// neighbours of the order, or the two groups at the border, are closer than the
+// scores' errors in 32 (kTol...): one token in a thousand. Rows that hold what is no
+// number go through choose_slowly.
 //
-// A workgroup takes a chunk of 32 tokens, L lanes a token (32, so that a chunk is in
-// flight at once; 64 from 513 experts on), each with C consecutive experts. A pick
-// is a maximum over the lanes (DPP and a lane swap, no LDS) and the first lane that
-// has it; that lane puts expert and score into LDS and looks for its next best.
-// Bound by the instructions of the picks, not by the logits' bytes.
+// A workgroup takes a chunk of 32 tokens, L lanes a token (16 up to 256 experts), each
+// with C consecutive experts, sorted by a network in its registers. A pick is a
+// maximum over the lanes' first ones (DPP, no LDS) and the first lane that has it; that
+// lane notes the expert and moves its list up. Bound by the instructions, about 1300 a
+// wave of four tokens of 256 experts, not by the logits' bytes.
 #include "moe_common.h"
 #include "moe_gemm.h"
 #include "route_list.h"
@@ -43,46 +44,73 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  const int i = __builtin_bit_cast(int, v);
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+// v of the lane that STEP says: 0, 1: 1 and 2 lanes apart; 2, 3: the halves of 8 and of
+// 16 mirrored; 4, 5: the other 16-lane row, the other 32-lane half (once v is alike
+// within these).
+template <int STEP>
+__device__ __forceinline__ unsigned other(unsigned v) {
+  if constexpr (STEP < 4) {
+    return dpp<STEP == 0 ? 0xB1 : STEP == 1 ? 0x4E : STEP == 2 ? 0x141 : 0x140>(v);
+  } else {
+    const auto r = [&] {
+      if constexpr (STEP == 4)
+        return __builtin_amdgcn_permlane16_swap(v, v, false, false);
+      else
+        return __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    }();
+    return r[0] ^ r[1] ^ v;  // (one of them is the lane's own)
+  }
+}
+template <int STEP>
+__device__ __forceinline__ int other(int v) {
+  return (int)other<STEP>((unsigned)v);
+}
+template <int STEP>
+__device__ __forceinline__ float other(float v) {
+  return __builtin_bit_cast(float, other<STEP>(__builtin_bit_cast(unsigned, v)));
+}
+template <int STEP>
+__device__ __forceinline__ double other(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t o = (uint64_t)other<STEP>((unsigned)(u >> 32)) << 32 | other<STEP>((unsigned)u);
+  return __builtin_bit_cast(double, o);
 }
 
-// op over the L lanes of a token, in every one of them: lanes 1 and 2 apart (quad
-// permutations), the halves of 8 and of 16 mirrored, then 16-lane rows and 32-lane
-// halves swapped. Needs the whole wave.
-template <int L, typename Op>
-__device__ __forceinline__ float reduce(float v, Op op) {
-  v = op(v, dpp<0xB1>(v));
-  v = op(v, dpp<0x4E>(v));
-  v = op(v, dpp<0x141>(v));
-  v = op(v, dpp<0x140>(v));
-  auto i = __builtin_bit_cast(unsigned, v);
-  const auto a = __builtin_amdgcn_permlane16_swap(i, i, false, false);
-  v = op(__builtin_bit_cast(float, (unsigned)a[0]), __builtin_bit_cast(float, (unsigned)a[1]));
-  if constexpr (L == 64) {
-    i = __builtin_bit_cast(unsigned, v);
-    const auto b = __builtin_amdgcn_permlane32_swap(i, i, false, false);
-    v = op(__builtin_bit_cast(float, (unsigned)b[0]), __builtin_bit_cast(float, (unsigned)b[1]));
-  }
+// op over the L lanes of a token, in every one of them. Needs the whole wave.
+template <int L, typename F, typename Op>
+__device__ __forceinline__ F reduce(F v, Op op) {
+  v = op(v, other<0>(v));
+  v = op(v, other<1>(v));
+  v = op(v, other<2>(v));
+  v = op(v, other<3>(v));
+  if constexpr (L >= 32) v = op(v, other<4>(v));
+  if constexpr (L >= 64) v = op(v, other<5>(v));
   return v;
 }
-template <int L>
-__device__ __forceinline__ float lanes_max(float v) {
-  return reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
+template <int L, typename F>
+__device__ __forceinline__ F lanes_max(F v) {
+  return reduce<L>(v, [](F a, F b) { return a > b ? a : b; });
 }
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
-  return reduce<L>(v, [](float a, float b) { return a + b; });
+template <int L, typename F>
+__device__ __forceinline__ F lanes_sum(F v) {
+  return reduce<L>(v, [](F a, F b) { return a + b; });
 }
 
-// The first lane of the token for which `yes` holds (lanes counted from the token's first; 32 or 64: none).
+// The token's lanes for which `yes` holds, from bit 0 on.
+template <int L>
+__device__ __forceinline__ uint64_t lanes_of(bool yes) {
+  const uint64_t m = __ballot(yes);
+  return L == 64 ? m : m >> (__lane_id() & (64 - L)) & ((1ull << (L & 63)) - 1);
+}
+// The first of them, or L.
 template <int L>
 __device__ __forceinline__ int first_lane(bool yes) {
-  const uint64_t m = __ballot(yes);
+  const uint64_t m = lanes_of<L>(yes);
   if constexpr (L == 64) return m != 0 ? __builtin_ctzll(m) : 64;
-  const uint32_t half = (__lane_id() & 32) != 0 ? (uint32_t)(m >> 32) : (uint32_t)m;
-  return half != 0 ? __builtin_ctz(half) : 32;
+  return __builtin_ctz((uint32_t)m | (L < 32 ? 1u << (L & 31) : 0u)) + (L == 32 && (uint32_t)m == 0 ? 32 : 0);
 }
 
 __device__ __forceinline__ void wave_sync() {
@@ -128,7 +156,7 @@ __device__ __forceinline__ double score_of(double l, bool softmax, double mx, do
 }
 
 // The choice of one token by a whole wave in 64 bits, for any logits and biases:
-// fills m.pick and, in m.score, 1, 0 where no live expert was left, or NaN in a row
+// fills m.pick and, in m.score, 0, -inf where no live expert was left, or NaN in a row
 // that holds no number. A call that keeps everything in LDS, so that its registers do not cost
 // the waves that never come here their places.
 template <typename T, typename Lds>
@@ -217,22 +245,199 @@ __device__ __attribute__((noinline)) void choose_slowly(const T* row, const floa
     if (sub == (at & 63)) {
       m.key[at] = kNone;
       m.pick[k] = at;
-      m.score[k] = poison ? NAN : best > kOff ? 1.0f : 0.0f;
+      m.score[k] = poison ? NAN : best > kOff ? 0.0f : -INFINITY;
     }
   }
   wave_sync();
 }
 
-// Bounds of the error of a difference of two scores (at most 1, each off by 4
-// roundings; softmax: by the sum's too, up to 21) plus biases, times two.
-constexpr float kTolSigmoid = 0x1p-20f, kTolSoftmax = 0x1p-18f, kTolBias = 0x1p-21f;
+// Bounds of the error of a difference of two scores: a sigmoid s from exp_near is off
+// by s (1 - s) (|l| 2^-24 + 2^-23) + s (2^-23 + 2^-24) < 2^-22, a softmax by up to 40
+// roundings of its sum and of 1 / sum more. Twice that, and of the biases' additions.
+constexpr float kTolSigmoid = 0x1p-20f, kTolSoftmax = 0x1p-18f, kTolBias = 0x1p-23f;
+
+// Whether two scores or values as near as a and b <= a may be the other way round.
+__device__ __forceinline__ bool near(float a, float b, float tol) {
+  return b > -INFINITY && a - b <= tol + kTolBias * (fabsf(a) + fabsf(b));
+}
+
+// The groups that stay (as bits; at most 64) from the experts' values (-inf: off). p
+// lanes share a group. `close`: the border lies between two that are near.
+template <int L, int C, typename F, typename Lds>
+__device__ __forceinline__ uint64_t groups_kept(const F (&value)[C], float tol, int sub, const astrai_moe_routing& opt,
+                                                int n_experts, Lds& m, bool& close) {
+  constexpr F kOffKey = (F)-INFINITY;
+  const int per = n_experts / opt.n_groups;
+  F* const values = reinterpret_cast<F*>(m.key);
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (sub * C + i < n_experts) values[sub * C + i] = value[i];
+  wave_sync();
+  int p = 1;
+  while (2 * p * opt.n_groups <= L) p *= 2;
+  const int g = sub / p;
+  F a1 = kOffKey, a2 = kOffKey;
+  if (g < opt.n_groups)
+    for (int j = sub & (p - 1); j < per; j += p) {
+      const F v = values[g * per + j];
+      const F low = v < a1 ? v : a1;
+      a2 = low > a2 ? low : a2;
+      a1 = v > a1 ? v : a1;
+    }
+  for (int off = 1; off < p; off *= 2) {
+    const F o1 = __shfl_xor(a1, off, L), o2 = __shfl_xor(a2, off, L);
+    const F low = o1 < a1 ? o1 : a1, high2 = o2 > a2 ? o2 : a2;
+    a2 = low > high2 ? low : high2;
+    a1 = o1 > a1 ? o1 : a1;
+  }
+  F mine = opt.group_top == 2 ? a1 + a2 : a1, last = kOffKey;
+  uint64_t kept = 0;
+  for (int k = 0; k < opt.topk_groups; ++k) {
+    last = lanes_max<L>(mine);
+    // (groups without live experts: the lowest not kept yet)
+    const int at = last > kOffKey ? first_lane<L>(mine == last) / p : __builtin_ctzll(~kept);
+    kept |= 1ull << at;
+    if (g == at) mine = kOffKey;
+  }
+  if (tol > 0.0f) close = near((float)last, (float)lanes_max<L>(mine), 2.0f * tol);
+  return kept;
+}
+
+// Whether the lane's i-th expert is in a group that stays.
+template <int C>
+__device__ __forceinline__ void in_kept(uint64_t kept, int sub, int per, bool (&in)[C]) {
+  int g = sub * C / per, left = per - (sub * C - g * per);
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    in[i] = (kept >> g & 1) != 0;
+    if (--left == 0) left = per, ++g;
+  }
+}
+
+// A float as an integer that orders alike; INT_MIN, below every float's, stands for
+// what is taken or does not exist.
+constexpr int kOff32 = INT32_MIN + 0x7fffff;  // -inf's
+__device__ __forceinline__ int order32(float v) {
+  const int i = __float_as_int(v + 0.0f);  // (-0 as 0)
+  return i ^ (i >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ float value32(int o) { return __int_as_float(o ^ (o >> 31 & 0x7fffffff)); }
+
+// Sorts a lane's C pairs (key above, ~index below) downwards: odd-even merges.
+template <int C>
+__device__ __forceinline__ void sort_down(uint64_t (&v)[C]) {
+#pragma unroll
+  for (int p = 1; p < C; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < C; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < C && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint64_t a = v[i + j], b = v[i + j + k];
+            const bool swap = b > a;
+            v[i + j] = swap ? b : a;
+            v[i + j + k] = swap ? a : b;
+          }
+}
+
+// The top_k experts of the largest keys (INT_MIN: none) into m.pick, their keys as
+// floats into m.score; dead ones (-inf) come last, by their index. Returns the largest
+// key left.
+template <int L, int C, typename Lds>
+__device__ __forceinline__ float pick(const int (&key)[C], int sub, int top_k, Lds& m) {
+  uint64_t v[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) v[i] = (uint64_t)((uint32_t)key[i] ^ 0x80000000u) << 32 | (uint32_t)~(sub * C + i);
+  sort_down(v);
+  for (int k = 0; k < top_k; ++k) {
+    const int mine = (int)((uint32_t)(v[0] >> 32) ^ 0x80000000u);
+    const int top = lanes_max<L>(mine);
+    if (sub == first_lane<L>(mine == top)) {
+      m.pick[k] = (int)~(uint32_t)v[0];
+      m.score[k] = value32(top);
+#pragma unroll
+      for (int i = 0; i + 1 < C; ++i) v[i] = v[i + 1];
+      v[C - 1] = 0;
+    }
+  }
+  const int left = lanes_max<L>((int)((uint32_t)(v[0] >> 32) ^ 0x80000000u));
+  return left <= kOff32 ? -INFINITY : value32(left);
+}
+
+// The same from 64-bit keys (-inf: off), for the few tokens that need them.
+template <int L, int C, typename Lds>
+__device__ __forceinline__ void pick64(double (&key)[C], int sub, int n_experts, int top_k, Lds& m) {
+  uint32_t open = 0;  // the lane's experts not chosen yet
+#pragma unroll
+  for (int i = 0; i < C; ++i) open |= sub * C + i < n_experts ? 1u << i : 0u;
+  for (int k = 0; k < top_k; ++k) {
+    double best = key[0];
+#pragma unroll
+    for (int i = 1; i < C; ++i) best = key[i] > best ? key[i] : best;
+    const double top = lanes_max<L>(best);
+    const bool live = top > -INFINITY;
+    if (sub == first_lane<L>(live ? best == top : open != 0)) {
+      int at = live ? 0 : __builtin_ctz(open);
+      if (live)
+#pragma unroll
+        for (int i = C - 1; i >= 0; --i) at = key[i] == top ? i : at;
+      m.pick[k] = sub * C + at;
+      m.score[k] = (float)top;
+      open &= ~(1u << at);
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        if (i == at) key[i] = -INFINITY;
+    }
+  }
+}
+
+// The lane's C of a row of n values from column c0 on, `none` behind its end. vec: rows
+// are whole 16-byte units on 16-byte boundaries.
+template <typename T, int C>
+__device__ __forceinline__ void load_run(const T* row, int c0, int n, bool vec, float none, float (&out)[C]) {
+  constexpr int V = C * sizeof(T) < 16 ? C : 16 / (int)sizeof(T);
+  struct alignas(V * sizeof(T)) Unit {
+    T v[V];
+  };
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < C; i += V) {
+      Unit u{};
+      const bool in = c0 + i < n;
+      if (in) u = *reinterpret_cast<const Unit*>(row + c0 + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[i + j] = in ? Elem<T>::to_f32(u.v[j]) : none;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) out[i] = c0 + i < n ? Elem<T>::to_f32(row[c0 + i]) : none;
+  }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+// exp on the hardware's exponential: off by |x| 2^-24 + 2^-23 of its value.
+__device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// Score of an expert in 32 bits (softmax: with the row's maximum and 1 / sum).
+__device__ __forceinline__ float score32(float l, bool softmax, float mx, float inv) {
+  return softmax ? expf(l - mx) * inv : 1.0f / (1.0f + expf(-l));
+}
+
+template <int L, bool kList>
+constexpr int score_threads() {  // a chunk at once where 32 L threads allow it
+  return kList || L > 32 ? kRouteThreads : ASTRAI_MOE_CHUNK_TOKENS * L;
+}
 
 template <typename T, typename W, int L, int C, bool kGroups, bool kList>
-__global__ __launch_bounds__(kRouteThreads, L * C <= 256 ? 8 : 4) void route_scores_kernel(
+__global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_kernel(
     const T* __restrict__ logits, const float* __restrict__ bias, const astrai_moe_routing opt, int64_t n_tokens,
     int n_experts, int top_k, int n_shared, int32_t* __restrict__ topk_idx, W* __restrict__ topk_w,
-    int32_t* __restrict__ chunk_hist, const RouteList list) {
-  constexpr int TOKENS = kRouteThreads / L;  // in flight
+    int32_t* __restrict__ chunk_hist, const RouteList list, bool vec, bool vec_bias) {
+  constexpr int THREADS = score_threads<L, kList>();
+  constexpr int TOKENS = THREADS / L < ASTRAI_MOE_CHUNK_TOKENS ? THREADS / L : ASTRAI_MOE_CHUNK_TOKENS;  // in flight
   __shared__ int hist[ASTRAI_MOE_MAX_EXPERTS];  // kList: the experts' first rows
   __shared__ TokenLds<L * C> lds[TOKENS];
   constexpr int kEntries = kList ? ASTRAI_MOE_CHUNK_TOKENS * ASTRAI_MOE_MAX_TOPK : 1;
@@ -245,32 +450,33 @@ __global__ __launch_bounds__(kRouteThreads, L * C <= 256 ? 8 : 4) void route_sco
   const int slots = top_k + n_shared, columns = n_experts + n_shared;
   if constexpr (kList) {
     const uint32_t all = n_tokens < 32 ? (1u << (int)n_tokens) - 1u : ~0u;
-    for (int e = threadIdx.x; e < columns; e += kRouteThreads) mask[e] = e < n_experts ? 0u : all;
+    for (int e = threadIdx.x; e < columns; e += THREADS) mask[e] = e < n_experts ? 0u : all;
   } else {
-    for (int e = threadIdx.x; e < n_experts; e += kRouteThreads) hist[e] = 0;
+    for (int e = threadIdx.x; e < n_experts; e += THREADS) hist[e] = 0;
   }
-  for (int i = threadIdx.x; i < (int)(t_end - t_begin) * n_shared; i += kRouteThreads) {
+  for (int i = threadIdx.x; i < (int)(t_end - t_begin) * n_shared; i += THREADS) {
     const int64_t at = (t_begin + i / n_shared) * slots + top_k + i % n_shared;
     (kList ? s_e : topk_idx)[at] = n_experts + i % n_shared;
     (kList ? s_w : topk_w)[at] = Elem<W>::from_f32(1.0f);
   }
   __syncthreads();
-  auto& m = lds[in_flight];
   const bool softmax = opt.score == ASTRAI_MOE_SCORE_SOFTMAX;
-  float b[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) b[i] = bias != nullptr && sub * C + i < n_experts ? bias[sub * C + i] : 0.0f;
+  const bool by_score = bias != nullptr || (kGroups && opt.group_top == 2);  // (otherwise the logits decide)
   for (int64_t t0 = t_begin; t0 < t_end; t0 += TOKENS) {
     const int64_t t = t0 + in_flight;
-    const bool on = t < t_end;
-    float l[C], s[C], key[C];
-    bool slow = false;
+    const bool on = t < t_end && in_flight < TOKENS;
+    if (__ballot(on) == 0) break;  // (none of the wave's tokens)
+    auto& m = lds[min(in_flight, TOKENS - 1)];
+    float l[C], b[C];
+    bool odd = kGroups && opt.n_groups > L;  // what is no finite number, or more groups than lanes
+    load_run<T, C>(logits + (on ? t : t_begin) * n_experts, sub * C, n_experts, vec, -INFINITY, l);
+    if (bias != nullptr)
+      load_run<float, C>(bias, sub * C, n_experts, vec_bias, 0.0f, b);
+    else
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int c = sub * C + i;
-      l[i] = c < n_experts ? (on ? Elem<T>::to_f32(logits[t * n_experts + c]) : 0.0f) : -INFINITY;
-      slow |= !(l[i] < INFINITY);
-    }
+      for (int i = 0; i < C; ++i) b[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) odd |= !(l[i] < INFINITY) || !(b[i] < INFINITY);
     float mx = l[0], inv = 1.0f;
     if (softmax) {
 #pragma unroll
@@ -278,122 +484,93 @@ __global__ __launch_bounds__(kRouteThreads, L * C <= 256 ? 8 : 4) void route_sco
       mx = lanes_max<L>(mx);
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        s[i] = expf(l[i] - mx);
-        sum += s[i];
-      }
+      for (int i = 0; i < C; ++i) sum += l[i] == -INFINITY ? 0.0f : exp_near(l[i] - mx);
       inv = 1.0f / lanes_sum<L>(sum);
+    }
+    const float tol = !by_score ? 0.0f : softmax ? kTolSoftmax : kTolSigmoid;
+    float value[C];  // what groups go by, and with a bias the experts
 #pragma unroll
-      for (int i = 0; i < C; ++i) s[i] *= inv;
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) s[i] = 1.0f / (1.0f + expf(-l[i]));
+    for (int i = 0; i < C; ++i) {
+      const bool off = l[i] == -INFINITY;
+      const float near_s = softmax ? exp_near(l[i] - mx) * inv : __builtin_amdgcn_rcpf(1.0f + exp_near(-l[i]));
+      value[i] = !by_score || off ? l[i] : near_s + b[i];
+    }
+    int key[C];
+    bool close = false, in[C];
+    uint64_t kept = 0;
+    if constexpr (kGroups) {
+      kept = groups_kept<L, C>(value, tol, sub, opt, n_experts, m, close);
+      in_kept<C>(kept, sub, n_experts / opt.n_groups, in);
     }
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      key[i] = bias == nullptr || l[i] == -INFINITY ? l[i] : s[i] + b[i];
-      slow |= !(key[i] < INFINITY);  // (NaN or +inf)
+      const int k = order32(bias == nullptr ? l[i] : value[i]);
+      key[i] = sub * C + i >= n_experts ? INT32_MIN : kGroups && !in[i] ? kOff32 : k;
     }
-    const float tol = softmax ? kTolSoftmax : kTolSigmoid;
-    if constexpr (kGroups) {
-      // P lanes share a group's experts; more groups than lanes go the other way
-      const int per = n_experts / opt.n_groups;
-      const bool by_score = bias == nullptr && opt.group_top == 2;
-      slow |= opt.n_groups > L;
-      float* const value_of_expert = reinterpret_cast<float*>(m.key);
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (sub * C + i < n_experts) value_of_expert[sub * C + i] = by_score && l[i] != -INFINITY ? s[i] : key[i];
-      wave_sync();
-      int p = 1;
-      while (2 * p * opt.n_groups <= L) p *= 2;
-      const int g = sub / p;
-      float a1 = -INFINITY, a2 = -INFINITY;
-      if (g < opt.n_groups)
-        for (int j = sub % p; j < per; j += p) {
-          const float v = value_of_expert[g * per + j];
-          a2 = fmaxf(a2, fminf(a1, v));
-          a1 = fmaxf(a1, v);
-        }
-      for (int off = 1; off < p; off *= 2) {
-        const float o1 = __shfl_xor(a1, off, L), o2 = __shfl_xor(a2, off, L);
-        a2 = fmaxf(fminf(a1, o1), fmaxf(a2, o2));
-        a1 = fmaxf(a1, o1);
-      }
-      float value = opt.group_top == 2 ? a1 + a2 : a1, last = 0.0f;
-      uint64_t kept = 0;
-      for (int k = 0; k < opt.topk_groups; ++k) {
-        last = lanes_max<L>(value);
-        const int at = first_lane<L>(value == last) / p;
-        kept |= 1ull << at;
-        if (g == at) value = -INFINITY;
-      }
-      const float next = lanes_max<L>(value);
-      slow |= !(last > -INFINITY);
-      // (one live expert of two, or the first of the groups left out as good as the last taken)
-      if (bias != nullptr || by_score) slow |= last - next <= 2.0f * (tol + kTolBias * (fabsf(last) + fabsf(next)));
-      int gi = sub * C / per, left = per - (sub * C - gi * per);
+    const float left_out = pick<L, C>(key, sub, top_k, m);
+    wave_sync();
+    if (bias != nullptr)
+      for (int k = sub; k < top_k; k += L)
+        close |= near(m.score[k], k + 1 < top_k ? m.score[k + 1] : left_out, tol);
+    if (__ballot(close && on) != 0) {  // (the wave's other tokens get the choice that they have)
+      double value64[C], key64[C], sum = 0.0;
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        if ((kept >> gi & 1) == 0) key[i] = -INFINITY;
-        if (--left == 0) left = per, ++gi;
+        const double x = l[i];
+        value64[i] = l[i] == -INFINITY ? 0.0 : softmax ? exp(x - (double)mx) : 1.0 / (1.0 + exp(-x));
+        sum += value64[i];
       }
-    }
-    // the picks: every lane's best, the lanes' best
-    float best = -INFINITY, best_s = 0.0f;
-    int best_i = 0;
-    auto look = [&]() {
-      best = key[0], best_s = s[0], best_i = 0;
+      if (softmax) sum = lanes_sum<L>(sum);
 #pragma unroll
-      for (int i = 1; i < C; ++i)
-        if (key[i] > best) best = key[i], best_s = s[i], best_i = i;
-    };
-    look();
-    float before = 0.0f;
-    const int rounds = bias != nullptr && top_k < n_experts ? top_k + 1 : top_k;  // (the first one left out too)
-    for (int k = 0; k < rounds; ++k) {
-      const float top = lanes_max<L>(best);
-      if (bias != nullptr && k > 0)
-        slow |= before - top <= tol + kTolBias * (fabsf(before) + fabsf(top)) && top > -INFINITY;
-      if (k == top_k) break;
-      slow |= !(top > -INFINITY);
-      before = top;
-      if (sub == first_lane<L>(best == top)) {
-        m.pick[k] = sub * C + best_i;
-        m.score[k] = best_s;
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-          if (i == best_i) key[i] = -INFINITY;
-        look();
+      for (int i = 0; i < C; ++i)
+        value64[i] = l[i] == -INFINITY ? -INFINITY
+                     : !by_score       ? (double)l[i]
+                                       : (softmax ? value64[i] / sum : value64[i]) + (double)b[i];
+      if constexpr (kGroups) {
+        kept = groups_kept<L, C>(value64, 0.0f, sub, opt, n_experts, m, close);
+        in_kept<C>(kept, sub, n_experts / opt.n_groups, in);
       }
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        key64[i] = kGroups && !in[i] ? -INFINITY : bias == nullptr ? (double)l[i] : value64[i];
+      pick64<L, C>(key64, sub, n_experts, top_k, m);
+      wave_sync();
     }
-    const uint64_t again = __ballot(slow && on);
-    wave_sync();
-    if (again != 0) {
+    const uint64_t odd_lanes = __ballot(odd && on);
+    if (odd_lanes != 0) {
       const int first = (threadIdx.x & ~63) / L;  // the wave's first token in flight
 #pragma unroll 1
       for (int h = 0; h < 64 / L; ++h)
-        if (L == 64 || (uint32_t)(again >> (32 * h)) != 0)
-          choose_slowly<T>(logits + (t0 + first + h) * n_experts, bias, &opt, n_experts,
-                                                      top_k, &lds[first + h]);
+        if ((odd_lanes >> (h * (L & 63)) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) != 0)
+          choose_slowly<T>(logits + (t0 + first + h) * n_experts, bias, &opt, n_experts, top_k, &lds[first + h]);
     }
-    float v = sub < top_k && on ? m.score[sub] : 0.0f;
-    if ((L == 64 ? again != 0 : (uint32_t)(again >> (threadIdx.x & 32)) != 0) && v == 1.0f) {
-      // a live pick's score in 32 bits, as the quick choice takes it
-      const float at = Elem<T>::to_f32(logits[t * n_experts + m.pick[sub]]);
-      v = softmax ? expf(at - mx) * inv : 1.0f / (1.0f + expf(-at));
+    // the weights, slots k = sub, sub + L, ...
+    constexpr int SLOTS = ASTRAI_MOE_MAX_TOPK > L ? ASTRAI_MOE_MAX_TOPK / L : 1;
+    float v[SLOTS], total = 0.0f;
+    int e[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int k = sub + i * L;
+      v[i] = 0.0f, e[i] = 0;
+      if (on && k < top_k) {
+        e[i] = m.pick[k];
+        const float got = m.score[k];  // NaN: the row holds no number; -inf: no live expert
+        v[i] = got == -INFINITY ? 0.0f : got != got ? got : score32(Elem<T>::to_f32(logits[t * n_experts + e[i]]), softmax, mx, inv);
+      }
+      total += v[i];
     }
-    const float total = lanes_sum<L>(v);
-    if (on && sub < top_k) {
-      const int e = m.pick[sub];
-      float w = opt.renormalise ? (total == 0.0f ? 0.0f : v / total) : v;
-      w *= opt.scale;
-      (kList ? s_e : topk_idx)[t * slots + sub] = e;
-      (kList ? s_w : topk_w)[t * slots + sub] = Elem<W>::from_f32(w);
+    total = lanes_sum<L>(total);
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int k = sub + i * L;
+      if (!on || k >= top_k) continue;
+      const float w = (opt.renormalise ? (total == 0.0f ? 0.0f : v[i] / total) : v[i]) * opt.scale;
+      (kList ? s_e : topk_idx)[t * slots + k] = e[i];
+      (kList ? s_w : topk_w)[t * slots + k] = Elem<W>::from_f32(w);
       if constexpr (kList)
-        atomicOr(&mask[e], 1u << (int)t);
+        atomicOr(&mask[e[i]], 1u << (int)t);
       else
-        atomicAdd(&hist[e], 1);
+        atomicAdd(&hist[e[i]], 1);
     }
   }
   __syncthreads();
@@ -401,7 +578,7 @@ __global__ __launch_bounds__(kRouteThreads, L * C <= 256 ? 8 : 4) void route_sco
     write_chunk_list<W>(mask, hist, s_e, s_w, (int)n_tokens, columns, slots, list);
     return;
   }
-  for (int e = threadIdx.x; e < columns; e += kRouteThreads)
+  for (int e = threadIdx.x; e < columns; e += THREADS)
     chunk_hist[(int64_t)blockIdx.x * columns + e] = e < n_experts ? hist[e] : (int)(t_end - t_begin);
 }
 
@@ -518,9 +695,12 @@ void launch_scores_cfg(const void* logits, const float* bias, const astrai_moe_r
   auto kernel = opt.n_groups > 1
                     ? (list != nullptr ? &route_scores_kernel<T, W, L, C, true, true> : &route_scores_kernel<T, W, L, C, true, false>)
                     : (list != nullptr ? &route_scores_kernel<T, W, L, C, false, true> : &route_scores_kernel<T, W, L, C, false, false>);
-  hipLaunchKernelGGL(kernel, grid, dim3(kRouteThreads), 0, s, static_cast<const T*>(logits), bias, opt, n_tokens,
-                     n_experts, top_k, n_shared, topk_idx, static_cast<W*>(topk_w), chunk_hist,
-                     list != nullptr ? *list : RouteList{});
+  const int threads = list != nullptr ? score_threads<L, true>() : score_threads<L, false>();
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, static_cast<const T*>(logits), bias, opt, n_tokens, n_experts,
+                     top_k, n_shared, topk_idx, static_cast<W*>(topk_w), chunk_hist,
+                     list != nullptr ? *list : RouteList{},
+                     n_experts * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0,
+                     n_experts % 4 == 0 && reinterpret_cast<uintptr_t>(bias) % 16 == 0);
 }
 
 template <typename T, typename W>
@@ -531,13 +711,13 @@ int launch_scores(const void* logits, const float* bias, const astrai_moe_routin
   launch_scores_cfg<T, W, L, C>(logits, bias, opt, n_tokens, n_experts, top_k, n_shared, topk_idx, topk_w,      \
                                 chunk_hist, list, s)
   if (n_experts <= 32)
-    ROUTE_CASE(32, 1);
+    ROUTE_CASE(16, 2);
   else if (n_experts <= 64)
-    ROUTE_CASE(32, 2);
+    ROUTE_CASE(16, 4);
   else if (n_experts <= 128)
-    ROUTE_CASE(32, 4);
+    ROUTE_CASE(16, 8);
   else if (n_experts <= 256)
-    ROUTE_CASE(32, 8);
+    ROUTE_CASE(16, 16);
   else if (n_experts <= 512)
     ROUTE_CASE(32, 16);
   else
