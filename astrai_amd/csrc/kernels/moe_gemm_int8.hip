@@ -66,7 +66,7 @@ struct Args {
   int kp, n, n_tiles_n, capacity;
   void* c;
   float* part;     // partial sums of a split last round, or null
-  int32_t* sched;  // run-time claims, or null
+  int32_t* sched;  // run-time claims (their counter cleared by the quantiser before), or null
 };
 
 // Per-tile global bases (bytes).
@@ -718,11 +718,6 @@ __global__ __launch_bounds__(64) void i8_split_reduce_kernel(const Args p, int G
                                                          t_rows, nt);
 }
 
-// Clears the run-time claim counter of a streaming launch.
-__global__ __launch_bounds__(64) void i8_sched_clear_kernel(int32_t* __restrict__ sched) {
-  if (threadIdx.x == 0) sched[0] = 0;
-}
-
 using SmallCfg = TileCfg<kMfmaSmallBM, 256, 4, 1, 4, 8>;
 using MidCfg = TileCfg<kMfmaMidBM, 256, 3, 2, 4, 8>;
 using Mid2Cfg = TileCfg<kMfmaMid2BM, 256, 3, 2, 4, 8>;
@@ -767,10 +762,6 @@ int launch_stream(const Int8Gemm& g, hipStream_t s) {
                    g.ws.bytes >= kSchedBytes + grid * (int64_t)sizeof(float) * kSplitUnitFloats
                ? reinterpret_cast<float*>(static_cast<char*>(g.ws.base) + kSchedBytes)
                : nullptr;
-  if (a.sched != nullptr) {
-    hipLaunchKernelGGL(i8_sched_clear_kernel, dim3(1), dim3(64), 0, s, a.sched);
-    if (int rc = check_launch("i8_sched_clear_kernel")) return rc;
-  }
   hipLaunchKernelGGL((gemm_i8_stream_kernel<T, kGateUp, kGather, kBias>), dim3((unsigned)grid), dim3(Cfg::THREADS), 0,
                      s, a);
   if (int rc = check_launch(kGateUp ? "gemm_i8_stream_kernel<gate_up>" : "gemm_i8_stream_kernel<down>")) return rc;

@@ -32,7 +32,9 @@ struct Int8Gemm {
   void* c;                // [*, n] dtype
   int64_t n_rows;
   int block_m;
-  GemmWorkspace ws;       // of the 256-row tiles, as the bf16 products'
+  // of the 256-row tiles, as the bf16 products'; its first int32, the counter of the
+  // run-time claims, is 0 (the quantiser of a clears it)
+  GemmWorkspace ws;
 };
 
 // silu(g) u of the sums of two products. An fp32 h is taken in 64 bits and rounded

@@ -62,13 +62,17 @@ struct ScaleOut {
   }
 };
 
+__device__ __forceinline__ uint32_t word_of(bf16_t v) { return v; }
+__device__ __forceinline__ uint32_t word_of(float v) { return __float_as_uint(v); }
+
 // One row per WAVES waves, held in registers between its maximum and its codes: a
 // thread has NV units of 8 columns, WAVES * 512 columns apart. kVec: rows start on
-// 16-byte boundaries. One read of x and one write of the codes, bound by these: 117 M
+// 16-byte boundaries. clear: a counter of the product that follows, set to 0. One read of x and one write of the codes, bound by these: 117 M
 // values of 8192 rows 100 us, 32768 rows of 14336 XX us (XX TB/s).
 template <typename T, int WAVES, int NV, bool kVec>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
-                                                            int64_t kp, int8_t* __restrict__ q, const ScaleOut out) {
+                                                            int64_t kp, int8_t* __restrict__ q, const ScaleOut out,
+                                                            int32_t* clear) {
   using C = typename CodeType<T>::type;
   constexpr int ROWS = 4 / WAVES;
   __shared__ float s_most[4];
@@ -77,29 +81,35 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   const bool on = r < n_rows;
   const T* const row = x + (on ? r : 0) * k;
   const int c0 = (WAVES == 1 ? lane : (int)threadIdx.x) * 8;
-  float v[NV][8];
-  float most = 0.0f;
+  if (clear != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *clear = 0;
+  constexpr int WORDS = 2 * sizeof(T);  // of a unit: values stay as they came, two bf16 a word
+  uint32_t v[NV][WORDS];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * WAVES * 512;
     if (kVec && c + 8 <= k && on) {
-      alignas(16) T in[8];
 #pragma unroll
-      for (int j = 0; j < 8; j += 16 / (int)sizeof(T))
-        *reinterpret_cast<uint4*>(in + j) = *reinterpret_cast<const uint4*>(row + c + j);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = Elem<T>::to_f32(in[j]);
+      for (int j = 0; j < WORDS; j += 4)
+        *reinterpret_cast<uint4*>(&v[i][j]) = *reinterpret_cast<const uint4*>(row + c + j * (4 / (int)sizeof(T)));
     } else {
+      T in[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = c + j < k && on ? Elem<T>::to_f32(row[c + j]) : 0.0f;
+      for (int j = 0; j < 8; ++j) in[j] = c + j < k && on ? row[c + j] : (T)0;
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j)
+        v[i][j] = sizeof(T) == 2 ? (uint32_t)word_of(in[2 * j]) | (uint32_t)word_of(in[(2 * j + 1) & 7]) << 16 : word_of(in[j & 7]);
     }
   }
+  auto value = [&](int i, int j) {  // the unit's j-th value as a float's bits
+    if constexpr (sizeof(T) == 2) return (j & 1) != 0 ? v[i][j / 2] & 0xffff0000u : v[i][j / 2] << 16;
+    else return v[i][j];
+  };
   // (as integers, which order the magnitudes of floats, NaN above infinity)
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) top = max(top, value(i, j) & 0x7fffffffu);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
   if constexpr (WAVES > 1) {
@@ -109,7 +119,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     for (int w = 0; w < WAVES; ++w) top = max(top, __float_as_uint(s_most[w]));
   }
   if (!on) return;
-  most = __uint_as_float(top);
+  const float most = __uint_as_float(top);
   const bool bad = top >= 0x7f800000u;
   if (WAVES == 1 || wave == 0) out.put(r, bad ? NAN : most / 127.0f, lane);
   const float shift = range_shift(most);
@@ -124,7 +134,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
       uint2 u;
     } o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o.b[j] = zero ? (int8_t)0 : (int8_t)code_of<C>((C)v[i][j] * (C)shift, m, inv);
+    for (int j = 0; j < 8; ++j) o.b[j] = zero ? (int8_t)0 : (int8_t)code_of<C>((C)__uint_as_float(value(i, j)) * (C)shift, m, inv);
     *reinterpret_cast<uint2*>(q + r * kp + c) = o.u;
   }
 }
@@ -133,9 +143,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
                                                                  int64_t kp, int8_t* __restrict__ q,
-                                                                 const ScaleOut out) {
+                                                                 const ScaleOut out, int32_t* clear) {
   using C = typename CodeType<T>::type;
   __shared__ uint32_t s_top[4];
+  if (clear != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *clear = 0;
   const int64_t r = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const T* const row = x + r * k;
@@ -165,39 +176,40 @@ __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __rest
 
 template <typename T, int WAVES, int NV>
 void launch_quantize_cfg(const void* x, bool vec, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out,
-                         hipStream_t s) {
+                         int32_t* clear, hipStream_t s) {
   hipLaunchKernelGGL((vec ? quantize_rows_kernel<T, WAVES, NV, true> : quantize_rows_kernel<T, WAVES, NV, false>),
                      dim3((unsigned)ceil_div(n_rows, 4 / WAVES)), dim3(256), 0, s, static_cast<const T*>(x), n_rows, k,
-                     int8_row_bytes(k), q, out);
+                     int8_row_bytes(k), q, out, clear);
 }
 
 // A wave per row up to 1024 columns, a workgroup beyond.
 template <typename T>
-int launch_quantize(const void* x, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out, hipStream_t s) {
+int launch_quantize(const void* x, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out, int32_t* clear,
+                    hipStream_t s) {
   const bool vec = k * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   if (k <= 512)
-    launch_quantize_cfg<T, 1, 1>(x, vec, n_rows, k, q, out, s);
+    launch_quantize_cfg<T, 1, 1>(x, vec, n_rows, k, q, out, clear, s);
   else if (k <= 1024)
-    launch_quantize_cfg<T, 1, 2>(x, vec, n_rows, k, q, out, s);
+    launch_quantize_cfg<T, 1, 2>(x, vec, n_rows, k, q, out, clear, s);
   else if (k <= 2048)
-    launch_quantize_cfg<T, 4, 1>(x, vec, n_rows, k, q, out, s);
+    launch_quantize_cfg<T, 4, 1>(x, vec, n_rows, k, q, out, clear, s);
   else if (k <= 4096)
-    launch_quantize_cfg<T, 4, 2>(x, vec, n_rows, k, q, out, s);
+    launch_quantize_cfg<T, 4, 2>(x, vec, n_rows, k, q, out, clear, s);
   else if (k <= 8192)
-    launch_quantize_cfg<T, 4, 4>(x, vec, n_rows, k, q, out, s);
+    launch_quantize_cfg<T, 4, 4>(x, vec, n_rows, k, q, out, clear, s);
   else if (k <= 16384)
-    launch_quantize_cfg<T, 4, 8>(x, vec, n_rows, k, q, out, s);
+    launch_quantize_cfg<T, 4, 8>(x, vec, n_rows, k, q, out, clear, s);
   else
     hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3((unsigned)n_rows), dim3(256), 0, s,
-                       static_cast<const T*>(x), n_rows, k, int8_row_bytes(k), q, out);
+                       static_cast<const T*>(x), n_rows, k, int8_row_bytes(k), q, out, clear);
   return check_launch("quantize_rows_kernel");
 }
 
 int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, int8_t* q, const ScaleOut& out,
-                         hipStream_t s) {
+                         int32_t* clear, hipStream_t s) {
   if (n_rows == 0) return ASTRAI_MOE_OK;
-  return dtype == ASTRAI_MOE_BF16 ? launch_quantize<bf16_t>(x, n_rows, k, q, out, s)
-                                  : launch_quantize<float>(x, n_rows, k, q, out, s);
+  return dtype == ASTRAI_MOE_BF16 ? launch_quantize<bf16_t>(x, n_rows, k, q, out, clear, s)
+                                  : launch_quantize<float>(x, n_rows, k, q, out, clear, s);
 }
 
 // The product for every shape: 64 x 64 tiles, 64 bytes of K staged at a time, four
@@ -303,7 +315,7 @@ int launch_general(const Int8Gemm& g, hipStream_t s) {
 // of up to 8 slots in flight at a time.
 template <typename T, int VW>
 __global__ __launch_bounds__(256) void sum_slots_kernel(const T* __restrict__ y, const int32_t* __restrict__ token_pos,
-                                                        const T* __restrict__ topk_w, int64_t n_tokens, int top_k,
+                                                        const T* __restrict__ row_w, int64_t n_tokens, int top_k,
                                                         int n_shared, int64_t dim, T* __restrict__ out) {
   struct alignas(VW * sizeof(T)) Vec {
     T v[VW];
@@ -320,8 +332,9 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(const T* __restrict__ y,
       for (int j = 0; j < 8; ++j) {
         w[j] = 0.0f;
         if (k0 + j < slots) {
-          w[j] = k0 + j < top_k ? Elem<T>::to_f32(topk_w[t * slots + k0 + j]) : part;
-          in[j] = *reinterpret_cast<const Vec*>(y + (int64_t)token_pos[t * slots + k0 + j] * dim + c);
+          const int row = token_pos[t * slots + k0 + j];
+          w[j] = k0 + j < top_k ? Elem<T>::to_f32(row_w[row]) : part;
+          in[j] = *reinterpret_cast<const Vec*>(y + (int64_t)row * dim + c);
         }
       }
 #pragma unroll
@@ -338,22 +351,22 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(const T* __restrict__ y,
 }
 
 template <typename T>
-int launch_sum_typed(const void* y, const int32_t* token_pos, const void* topk_w, int64_t n_tokens, int top_k,
+int launch_sum_typed(const void* y, const int32_t* token_pos, const void* row_w, int64_t n_tokens, int top_k,
                      int n_shared, int64_t dim, void* out, hipStream_t s) {
   constexpr int kVW = 16 / sizeof(T);
   const bool vec = dim % kVW == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;  // (y is the workspace's)
   const dim3 grid((unsigned)n_tokens, (unsigned)std::min<int64_t>(ceil_div(dim, 256 * (vec ? kVW : 1)), 64));
   hipLaunchKernelGGL((vec ? sum_slots_kernel<T, kVW> : sum_slots_kernel<T, 1>), grid, dim3(256), 0, s,
-                     static_cast<const T*>(y), token_pos, static_cast<const T*>(topk_w), n_tokens, top_k, n_shared, dim,
+                     static_cast<const T*>(y), token_pos, static_cast<const T*>(row_w), n_tokens, top_k, n_shared, dim,
                      static_cast<T*>(out));
   return check_launch("sum_slots_kernel");
 }
 
-int launch_sum_slots(const void* y, const int32_t* token_pos, const void* topk_w, int dtype, int64_t n_tokens,
+int launch_sum_slots(const void* y, const int32_t* token_pos, const void* row_w, int dtype, int64_t n_tokens,
                      int top_k, int n_shared, int64_t dim, void* out, hipStream_t s) {
   return dtype == ASTRAI_MOE_BF16
-             ? launch_sum_typed<bf16_t>(y, token_pos, topk_w, n_tokens, top_k, n_shared, dim, out, s)
-             : launch_sum_typed<float>(y, token_pos, topk_w, n_tokens, top_k, n_shared, dim, out, s);
+             ? launch_sum_typed<bf16_t>(y, token_pos, row_w, n_tokens, top_k, n_shared, dim, out, s)
+             : launch_sum_typed<float>(y, token_pos, row_w, n_tokens, top_k, n_shared, dim, out, s);
 }
 
 int check_int8(const char* who, int dtype, int64_t k, int64_t n) {
@@ -486,7 +499,8 @@ extern "C" int astrai_moe_quantize_rows(const void* x, int dtype, int64_t n_rows
   if (n_rows == 0) return ASTRAI_MOE_OK;
   ASTRAI_REQUIRE(x && q && scale, "quantize_rows: null buffer");
   ASTRAI_REQUIRE(on16(q), "quantize_rows: q must start on a 16-byte boundary");
-  return launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, static_cast<hipStream_t>(stream));
+  return launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, nullptr,
+                              static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t astrai_moe_int8_linear_workspace_bytes(int64_t n_rows, int64_t k, int64_t n, int dtype) {
@@ -513,7 +527,8 @@ extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
   char* const base = static_cast<char*>(workspace);
   int8_t* const q = reinterpret_cast<int8_t*>(base + p.q);
   float* const scale = reinterpret_cast<float*>(base + p.scale);
-  if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, s)) return rc;
+  int32_t* const claims = p.gemm_ws_bytes > 0 ? reinterpret_cast<int32_t*>(base + p.gemm_ws) : nullptr;
+  if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, claims, s)) return rc;
   Int8Gemm g{RowCounts(n_rows, 1)};
   g.a = q, g.a_scale = scale, g.w0 = w, g.s0 = w_scale, g.bias = bias;
   g.kp = int8_row_bytes(k), g.n = n, g.dtype = dtype, g.c = out;
@@ -560,18 +575,28 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
   auto i8 = [&](int64_t off) { return reinterpret_cast<int8_t*>(base + off); };
   auto f32 = [&](int64_t off) { return reinterpret_cast<float*>(base + off); };
   int32_t *const topk_idx = i32(p.topk_idx), *const hist = i32(p.chunk_hist), *const tiles = i32(p.tiles);
-  if (routing != nullptr)
-    rc = launch_route_scores(logits, logits_dtype, bias, *routing, n_tokens, n_experts, top_k, n_shared, dtype,
-                             topk_idx, base + p.topk_w, hist, s);
-  else
-    rc = launch_route(logits, dtype, n_tokens, n_experts, top_k, n_shared, topk_idx, base + p.topk_w, hist, s);
-  if (rc) return rc;
-  if ((rc = astrai_moe_permute(topk_idx, base + p.topk_w, hist, nullptr, dtype, n_tokens, p.experts, p.slots, p.dp / 2,
-                               p.block_m, i32(p.offsets), i32(p.sorted_token), base + p.sorted_w, i32(p.token_pos),
-                               nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
-    return rc;
+  int32_t* const claims = p.gemm_ws_bytes > 0 ? i32(p.gemm_ws) : nullptr;
+  // One chunk of tokens: routing and permutation in one workgroup.
+  if (n_tokens <= ASTRAI_MOE_CHUNK_TOKENS) {
+    const RouteList list{i32(p.sorted_token), base + p.sorted_w, i32(p.token_pos), tiles,
+                         (p.tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE, p.block_m};
+    rc = routing != nullptr ? launch_route_scores_list(logits, logits_dtype, bias, *routing, n_tokens, n_experts, top_k,
+                                                       n_shared, dtype, list, s)
+                            : launch_route_list(logits, dtype, n_tokens, n_experts, top_k, n_shared, list, s);
+    if (rc) return rc;
+  } else {
+    rc = routing != nullptr
+             ? launch_route_scores(logits, logits_dtype, bias, *routing, n_tokens, n_experts, top_k, n_shared, dtype,
+                                   topk_idx, base + p.topk_w, hist, s)
+             : launch_route(logits, dtype, n_tokens, n_experts, top_k, n_shared, topk_idx, base + p.topk_w, hist, s);
+    if (rc) return rc;
+    if ((rc = astrai_moe_permute(topk_idx, base + p.topk_w, hist, nullptr, dtype, n_tokens, p.experts, p.slots, p.dp / 2,
+                                 p.block_m, i32(p.offsets), i32(p.sorted_token), base + p.sorted_w, i32(p.token_pos),
+                                 nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
+      return rc;
+  }
   if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq),
-                                 ScaleOut{f32(p.xs), i32(p.token_pos), p.slots}, s))) return rc;
+                                 ScaleOut{f32(p.xs), i32(p.token_pos), p.slots}, claims, s))) return rc;
   Int8Gemm g{row_counts(z)};
   if (p.gemm_ws_bytes > 0) g.ws = {base + p.gemm_ws, p.gemm_ws_bytes};
   g.a = i8(p.xq), g.a_scale = f32(p.xs), g.row_src = i32(p.sorted_token);
@@ -581,10 +606,10 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
   g.kp = p.dp, g.n = dim_ffn, g.dtype = dtype, g.c = base + p.h, g.block_m = p.block_m;
   if ((rc = launch_int8_gemm(g, s))) return rc;
   if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq),
-                                 ScaleOut{f32(p.hs), nullptr, 0}, s))) return rc;
+                                 ScaleOut{f32(p.hs), nullptr, 0}, claims, s))) return rc;
   g.a = i8(p.hq), g.a_scale = f32(p.hs), g.row_src = nullptr;
   g.w0 = w_down, g.w1 = nullptr, g.s0 = down_scale, g.s1 = nullptr;
   g.kp = p.fp, g.n = dim, g.c = base + p.y;
   if ((rc = launch_int8_gemm(g, s))) return rc;
-  return launch_sum_slots(base + p.y, i32(p.token_pos), base + p.topk_w, dtype, n_tokens, top_k, n_shared, dim, out, s);
+  return launch_sum_slots(base + p.y, i32(p.token_pos), base + p.sorted_w, dtype, n_tokens, top_k, n_shared, dim, out, s);
 }
