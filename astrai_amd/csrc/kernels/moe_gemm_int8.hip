@@ -41,6 +41,7 @@ struct RowTiles {
   __device__ int live(int capacity) const {
     return tiles == nullptr ? capacity : min(tiles[0], min(tiles[2], capacity));
   }
+  __device__ int height() const { return tiles == nullptr ? block_m : tiles[1]; }
   __device__ void get(int mt, int& e, int& row0, int& end) const {
     if (tiles == nullptr) {
       e = 0;
@@ -724,6 +725,233 @@ using Mid2Cfg = TileCfg<kMfmaMid2BM, 256, 3, 2, 4, 8>;
 using NarrowCfg = TileCfg<kMfmaMid2BM, 128, 4, 4, 2, 8>;
 using NarrowMidCfg = TileCfg<kMfmaMidBM, 128, 3, 2, 2, 8>;
 
+#if ASTRAI_MOE_RAGGED_K
+// ===========================================================================
+// Few rows: as gemm_few_kernel of moe_gemm_few.hip, bound by reading the weights
+// once with every compute unit. A column tile is 32 or 16 weight rows; the four waves
+// of a workgroup take every fourth K step of it, each through an LDS ring of its own,
+// and their sums meet in LDS, 32 rows at a time. (For every shape: whole K steps gain
+// nothing here.)
+// ===========================================================================
+template <int BM_, int BN_>
+struct FewCfg {
+  static constexpr int BM = BM_, BN = BN_, WAVES = 4, STAGES = BM == 64 ? 3 : BN == 32 ? 4 : 6;
+  static constexpr int NR = BM / 16, NC = BN / 16;  // 16-row and 16-column blocks
+  static constexpr int A_BYTES = BM * kRowBytes, B_BYTES = BN * kRowBytes, STAGE = A_BYTES + B_BYTES;
+  static constexpr int OPS = STAGE / 1024;                     // DMA ops per wave and step
+  static constexpr int RED_ROWS = 32;                          // rows whose sums meet at a time
+  static constexpr int RED_WAVE = RED_ROWS * BN * 4;           // one wave's sums of these
+  static constexpr int RED_OFF = WAVES * STAGES * STAGE;       // 128 or 144 KB of rings
+  static constexpr int RED_BUFS = BM == 64 ? 1 : 2;            // places they meet in
+  static constexpr int LDS = RED_OFF + RED_BUFS * WAVES * RED_WAVE;  // 160 KB
+  static_assert(LDS <= 160 * 1024, "LDS");
+  static_assert(OPS * (STAGES - 1) <= 63, "vmcnt range");
+};
+
+// Position of a wave in its sequence of K steps: run `sub` of BM rows of tile `unit`,
+// the wave's step j of n.
+template <typename Cfg, bool kGateUp, bool kGather>
+struct FewCursor {
+  int unit, mt, nt, e, row0, rows, sub, j, n, rot;
+  bool live;
+  const char *a, *b0, *b1;
+  uint32_t off[Cfg::BM / 8];  // byte offsets of the rows a lane loads of the activation tile
+  int b_rows;
+
+  __device__ void enter(const Args& p) {
+    constexpr int kCols = kGateUp ? Cfg::BN / 2 : Cfg::BN;
+    mt = unit / p.n_tiles_n;
+    nt = unit - mt * p.n_tiles_n;
+    int end;
+    p.tiles.get(mt, e, row0, end);
+    e = uniform(e), row0 = uniform(row0);
+    rows = min(uniform(p.tiles.height()), uniform(end) - row0);
+    b_rows = min(kCols, p.n - nt * kCols);
+    const int64_t at = ((int64_t)e * p.n + (int64_t)nt * kCols) * p.kp;
+    b0 = reinterpret_cast<const char*>(p.w0 + at);
+    b1 = kGateUp ? reinterpret_cast<const char*>(p.w1 + at) : b0;
+    rot = n > 0 ? (7 * e + 3 * nt) % n : 0;
+    sub = 0;
+  }
+  __device__ void enter_rows(const Args& p, int lane) {
+    j = 0;
+    a = reinterpret_cast<const char*>(kGather ? p.a : p.a + (int64_t)(row0 + sub * Cfg::BM) * p.kp);
+    const int last = rows - sub * Cfg::BM - 1;  // pad rows re-read the last row
+#pragma unroll
+    for (int q = 0; q < Cfg::BM / 8; ++q) {
+      const int r = min(q * 8 + (lane >> 3), last);
+      off[q] = (kGather ? (uint32_t)p.row_src[row0 + sub * Cfg::BM + r] : (uint32_t)r) * (uint32_t)p.kp;
+    }
+  }
+  __device__ void advance(const Args& p, int total, int G, int lane) {
+    if (++j < n) return;
+    const int old_mt = mt, old_sub = sub;
+    if ((sub + 1) * Cfg::BM < rows) {
+      ++sub;
+    } else {
+      unit += G;
+      live = unit < total;
+      if (!live) return;
+      enter(p);
+    }
+    if (mt == old_mt && sub == old_sub)
+      j = 0;
+    else
+      enter_rows(p, lane);
+  }
+  // the wave's next step into LDS at `lds`
+  __device__ void issue(const Args& p, int wave, int lane, char* lds) const {
+    int jr = j + rot;
+    if (jr >= n) jr -= n;
+    const int ks = wave + Cfg::WAVES * jr;
+    const uint32_t kp = (uint32_t)p.kp;
+    const DmaLane dl(lane, ks);
+    const bool tail = (uint32_t)(ks + 1) * kRowBytes > kp;
+#pragma unroll
+    for (int q = 0; q < Cfg::BM / 8; ++q) {
+      if (tail)
+        dma_16_or_zero(a, off[q] + dl.chunk(q), dl.chunk(q), kp, lds + q * 1024);
+      else
+        lds_dma_16(a + (off[q] + dl.chunk(q)), lds + q * 1024);
+    }
+    lds += Cfg::A_BYTES;
+#pragma unroll
+    for (int q = 0; q < Cfg::BN / 8; ++q) {
+      constexpr int kHalf = Cfg::BN / 16;  // gate/up: ops of the gate rows, then of the up rows
+      const char* b = kGateUp && q >= kHalf ? b1 : b0;
+      const int q_in = kGateUp ? q % kHalf : q;
+      const uint32_t o = (uint32_t)min(q_in * 8 + dl.row, b_rows - 1) * kp + dl.chunk(q);
+      if (tail)
+        dma_16_or_zero(b, o, dl.chunk(q), kp, lds + q * 1024);
+      else
+        lds_dma_16(b + o, lds + q * 1024);
+    }
+  }
+};
+
+template <typename Cfg, typename T, bool kGateUp, bool kGather>
+__global__ __launch_bounds__(Cfg::WAVES * 64, 1) void gemm_i8_few_kernel(const Args p) {
+  constexpr int NR = Cfg::NR, NC = Cfg::NC;
+  __shared__ __attribute__((aligned(1024))) char smem[Cfg::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int G = gridDim.x;
+  const int total = uniform(p.tiles.live(p.capacity)) * p.n_tiles_n;
+  if ((int)blockIdx.x >= total) return;
+  char* const ring = smem + wave * (Cfg::STAGES * Cfg::STAGE);
+
+  FewCursor<Cfg, kGateUp, kGather> ld;  // the next step to load
+  const int KT = (p.kp + kRowBytes - 1) / kRowBytes;
+  const int n_steps = KT > wave ? (KT - wave + Cfg::WAVES - 1) / Cfg::WAVES : 0;
+  ld.n = n_steps;
+  ld.unit = blockIdx.x;
+  ld.enter(p);
+  ld.enter_rows(p, lane);
+  ld.live = n_steps > 0;
+  int issued = 0, used = 0;  // steps loaded and consumed so far; step i sits in stage i % STAGES
+  auto issue = [&]() {
+    ld.issue(p, wave, lane, ring + (issued % Cfg::STAGES) * Cfg::STAGE);
+    ++issued;
+    ld.advance(p, total, G, lane);
+  };
+#pragma unroll 1
+  for (int i = 0; i < Cfg::STAGES; ++i)
+    if (ld.live) issue();
+
+  const int frag_row = lane & 15, fq = lane >> 4, fsw = (frag_row >> 1) & 7;
+  int parity = 0;
+  for (int unit = blockIdx.x; unit < total; unit += G) {
+    const int mt = unit / p.n_tiles_n, nt = unit - mt * p.n_tiles_n;
+    int e, row0, end;
+    p.tiles.get(mt, e, row0, end);
+    const int rows = uniform(min(p.tiles.height(), end - row0));
+    for (int r0 = 0; r0 < rows; r0 += Cfg::BM) {
+      i32x4_t acc[NR][NC];
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[i][c] = i32x4_t{0, 0, 0, 0};
+      for (int step = 0; step < n_steps; ++step) {
+        wait_groups<Cfg::OPS, Cfg::STAGES - 1>(issued - used - 1);  // this step has landed
+        const char* sa = ring + (used % Cfg::STAGES) * Cfg::STAGE + frag_row * kRowBytes;
+        i32x4_t fa[2][NR], fb[2][NC];
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          const int chunk = ((kh * 4 + fq) ^ fsw) << 4;
+#pragma unroll
+          for (int i = 0; i < NR; ++i)
+            fa[kh][i] = *reinterpret_cast<const i32x4_t*>(sa + i * 16 * kRowBytes + chunk);
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            fb[kh][c] = *reinterpret_cast<const i32x4_t*>(sa + Cfg::A_BYTES + c * 16 * kRowBytes + chunk);
+        }
+        wait_lds();  // the stage has been read: it may be loaded again
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        ++used;
+        if (ld.live) issue();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              acc[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[kh][c], fa[kh][i], acc[i][c], 0, 0, 0);
+      }
+      // the waves' sums meet, 32 rows at a time: row r's 16-byte piece c at piece
+      // c ^ (r % pieces)
+      static_for<Cfg::BM / Cfg::RED_ROWS>([&](auto half) {
+        constexpr int i0 = decltype(half)::value * 2;  // the first of these rows' two 16-row blocks
+        const int rh = r0 + i0 * 16;
+        if (rh >= rows) return;
+        constexpr int PIECES = Cfg::BN / 4, ROW = Cfg::BN * 4;
+        char* const red = smem + Cfg::RED_OFF + parity * (Cfg::WAVES * Cfg::RED_WAVE);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const int r = i * 16 + frag_row;
+            *reinterpret_cast<i32x4_t*>(red + wave * Cfg::RED_WAVE + r * ROW +
+                                        (((c * 4 + fq) ^ (r & (PIECES - 1))) << 4)) = acc[i0 + i][c];
+          }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        auto sum = [&](int r, int piece) {
+          i32x4_t v = {0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < Cfg::WAVES; ++w)
+            v += *reinterpret_cast<const i32x4_t*>(red + w * Cfg::RED_WAVE + r * ROW + ((piece ^ (r & (PIECES - 1))) << 4));
+          return v;
+        };
+        constexpr int CP = kGateUp ? PIECES / 2 : PIECES;  // pieces of output columns
+        const int r = threadIdx.x / CP, c = threadIdx.x % CP, n = nt * (CP * 4) + c * 4;
+        if (r < Cfg::RED_ROWS && rh + r < rows && n < p.n) {
+          const int64_t row = row0 + rh + r;
+          const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+          const f32x4_t s0 = four(p.s0, e, n, p.n), s1 = kGateUp ? four(p.s1, e, n, p.n) : zero;
+          const f32x4_t bias = !kGateUp && p.bias != nullptr ? bias_of<T>(p.bias, n, p.n) : zero;
+          const i32x4_t g = sum(r, c);
+          const auto o = out_of<T, kGateUp>(g, kGateUp ? sum(r, CP + c) : g, p.a_scale[row], s0, s1, bias);
+          using E = std::conditional_t<std::is_same_v<T, bf16_t>, __bf16, T>;
+          E* const at = static_cast<E*>(p.c) + row * p.n + n;
+          if (p.n % 4 == 0) {
+            *reinterpret_cast<typename Out4<T>::type*>(at) = o;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (n + q < p.n) at[q] = o[q];
+          }
+        }
+        if constexpr (Cfg::RED_BUFS == 2)
+          parity ^= 1;
+        else  // the next sums go to the same place
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      });
+    }
+  }
+}
+#endif  // ASTRAI_MOE_RAGGED_K
+
 Args args_of(const Int8Gemm& g) {
   Args a{};
   a.a = g.a, a.a_scale = g.a_scale, a.row_src = g.row_src;
@@ -795,14 +1023,54 @@ int launch_typed(const Int8Gemm& g, hipStream_t s) {
   return launch_tiles<SmallCfg, T, kGateUp, kGather>(g, s);
 }
 
+#if ASTRAI_MOE_RAGGED_K
+template <typename Cfg, typename T, bool kGateUp, bool kGather>
+int launch_few_cfg(const Int8Gemm& g, hipStream_t s) {
+  if (g.capacity == 0) return ASTRAI_MOE_OK;
+  Args a = args_of(g);
+  const int64_t n_cols = ceil_div(g.n, kGateUp ? Cfg::BN / 2 : Cfg::BN);  // the last may be partial
+  a.n_tiles_n = (int)n_cols;
+  int64_t grid = 0;
+  if (int rc = persistent_grid(g.capacity, n_cols, &grid)) return rc;
+  hipLaunchKernelGGL((gemm_i8_few_kernel<Cfg, T, kGateUp, kGather>), dim3((unsigned)grid), dim3(Cfg::WAVES * 64), 0, s, a);
+  return check_launch(kGateUp ? "gemm_i8_few_kernel<gate_up>" : "gemm_i8_few_kernel<down>");
+}
+
+// Tiles of 64 rows where lists are as high and most experts, or one, have more than
+// 32; of 16 weight rows for one expert's single run of rows where these fill the
+// compute units better (the rules of launch_few_tiles in moe_gemm_few.hip).
+template <typename T, bool kGateUp, bool kGather>
+int launch_few(const Int8Gemm& g, hipStream_t s) {
+  const int64_t most = g.rows.dense() ? 2 * FewCfg<32, 32>::BM : 24 * (int64_t)(g.rows.experts + g.rows.exact);
+  if (g.block_m >= FewCfg<64, 32>::BM && g.rows.total() > most)
+    return launch_few_cfg<FewCfg<64, 32>, T, kGateUp, kGather>(g, s);
+  auto fill = [](int64_t tiles) {  // share of the compute units' time that they fill
+    const double rounds = (double)tiles / cu_count();
+    return rounds / std::ceil(rounds);
+  };
+  if (g.rows.dense() && g.rows.total() <= FewCfg<32, 16>::BM &&
+      fill(ceil_div(g.n, kGateUp ? 8 : 16)) > 1.05 * fill(ceil_div(g.n, kGateUp ? 16 : 32)))
+    return launch_few_cfg<FewCfg<32, 16>, T, kGateUp, kGather>(g, s);
+  return launch_few_cfg<FewCfg<32, 32>, T, kGateUp, kGather>(g, s);
+}
+#endif
+
 }  // namespace
 
 #if ASTRAI_MOE_RAGGED_K
 namespace ragged {
+
+int launch_int8_few(const Int8Gemm& g, hipStream_t s) {
+  if (g.dtype == ASTRAI_MOE_BF16)
+    return g.w1 != nullptr ? launch_few<bf16_t, true, true>(g, s) : launch_few<bf16_t, false, false>(g, s);
+  return g.w1 != nullptr ? launch_few<float, true, true>(g, s) : launch_few<float, false, false>(g, s);
+}
+
 #endif
 
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s) {
 #if !ASTRAI_MOE_RAGGED_K
+  if (aligned16(g.c) && few_rows(g.rows, g.block_m, g.kp / 2, g.n, g.w1 != nullptr)) return ragged::launch_int8_few(g, s);
   const int size = g.dtype == ASTRAI_MOE_BF16 ? 2 : 4;
   if (g.kp % kRowBytes != 0 || g.n * size % 16 != 0 || g.n % 4 != 0 || !aligned16(g.c))
     return ragged::launch_int8_mfma(g, s);

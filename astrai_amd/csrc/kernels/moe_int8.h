@@ -64,6 +64,7 @@ int launch_int8_gemm(const Int8Gemm& g, hipStream_t s);
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
 namespace ragged {
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
+int launch_int8_few(const Int8Gemm& g, hipStream_t s);  // few rows (few_rows), every shape; c aligned
 }
 
 }  // namespace astrai_moe
