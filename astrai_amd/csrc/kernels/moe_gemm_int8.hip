@@ -64,6 +64,9 @@ struct Args {
   const int8_t *w0, *w1;
   const float *s0, *s1;
   const void* bias;
+  const void* x;  // rows to quantise in the kernel, their columns, and whether they are aligned to 16 bytes
+  int64_t k;
+  bool vec;
   int kp, n, n_tiles_n, capacity;
   void* c;
   float* part;     // partial sums of a split last round, or null
@@ -950,6 +953,233 @@ __global__ __launch_bounds__(Cfg::WAVES * 64, 1) void gemm_i8_few_kernel(const A
     }
   }
 }
+
+// ===========================================================================
+// A few tokens: the product quantises its rows itself. Every workgroup reads the (at
+// most 16) rows of its row tile, whose codes stay in LDS, behind its first weight
+// loads: for one token the launch and the trip through memory that a quantiser of its
+// own takes (4 to 5 us) are most of a small product's time. Otherwise as above.
+// ===========================================================================
+struct QuantCfg {
+  static constexpr int BM = 16, BN = 32, WAVES = 4, STAGES = 8, UNITS = 2;
+  static constexpr int STAGE = BN * kRowBytes;                 // weights only
+  static constexpr int CODES = UNITS * WAVES * 512 + BM * kRowBytes;  // bytes of the rows' codes, in whole steps
+  static constexpr int RED_WAVE = BM * BN * 4;                 // one wave's sums
+  static constexpr int CODE_OFF = WAVES * STAGES * STAGE, RED_OFF = CODE_OFF + CODES;
+  static constexpr int LDS = RED_OFF + 2 * WAVES * RED_WAVE;   // 150 KB
+  static_assert(LDS + 256 <= 160 * 1024, "LDS");
+};
+
+template <typename T, bool kGateUp, bool kGather>
+__global__ __launch_bounds__(QuantCfg::WAVES * 64, 1) void gemm_i8_quant_kernel(const Args p) {
+  using Cfg = QuantCfg;
+  using C = typename CodeType<T>::type;
+  constexpr int NC = Cfg::BN / 16, OPS = Cfg::STAGE / 1024;
+  __shared__ __attribute__((aligned(1024))) char smem[Cfg::LDS];
+  __shared__ uint32_t s_top[Cfg::BM];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int G = gridDim.x;
+  const int total = uniform(p.tiles.live(p.capacity)) * p.n_tiles_n;
+  if ((int)blockIdx.x >= total) return;
+  char* const ring = smem + wave * (Cfg::STAGES * Cfg::STAGE);
+  char* const codes = smem + Cfg::CODE_OFF;
+  const uint32_t kp = (uint32_t)p.kp;
+  const int KT = (p.kp + kRowBytes - 1) / kRowBytes, row_bytes = KT * kRowBytes;
+  const int n_steps = KT > wave ? (KT - wave + Cfg::WAVES - 1) / Cfg::WAVES : 0;
+  constexpr int kCols = kGateUp ? Cfg::BN / 2 : Cfg::BN;
+
+  // ---- weights: the wave's next step to load ----
+  int l_unit = blockIdx.x, l_j = 0, l_rot = 0, l_rows = 0;
+  bool l_live = n_steps > 0;
+  const char *b0 = nullptr, *b1 = nullptr;
+  auto enter = [&]() {
+    const int mt = l_unit / p.n_tiles_n, nt = l_unit - mt * p.n_tiles_n;
+    int e, row0, end;
+    p.tiles.get(mt, e, row0, end);
+    e = uniform(e);
+    l_rows = min(kCols, p.n - nt * kCols);
+    const int64_t at = ((int64_t)e * p.n + (int64_t)nt * kCols) * p.kp;
+    b0 = reinterpret_cast<const char*>(p.w0 + at);
+    b1 = kGateUp ? reinterpret_cast<const char*>(p.w1 + at) : b0;
+    l_rot = n_steps > 0 ? (7 * e + 3 * nt) % n_steps : 0;
+    l_j = 0;
+  };
+  int issued = 0, used = 0;
+  auto issue = [&]() {
+    int jr = l_j + l_rot;
+    if (jr >= n_steps) jr -= n_steps;
+    const int ks = wave + Cfg::WAVES * jr;
+    char* const lds = ring + (issued % Cfg::STAGES) * Cfg::STAGE;
+    const DmaLane dl(lane, ks);
+    const bool tail = (uint32_t)(ks + 1) * kRowBytes > kp;
+#pragma unroll
+    for (int q = 0; q < OPS; ++q) {
+      constexpr int kHalf = OPS / 2;
+      const char* b = kGateUp && q >= kHalf ? b1 : b0;
+      const int q_in = kGateUp ? q % kHalf : q;
+      const uint32_t o = (uint32_t)min(q_in * 8 + dl.row, l_rows - 1) * kp + dl.chunk(q);
+      if (tail)
+        dma_16_or_zero(b, o, dl.chunk(q), kp, lds + q * 1024);
+      else
+        lds_dma_16(b + o, lds + q * 1024);
+    }
+    ++issued;
+    if (++l_j == n_steps) {
+      l_unit += G;
+      l_live = l_unit < total;
+      if (l_live) enter();
+    }
+  };
+  enter();
+
+  // ---- the rows of one tile: unit i of the wave is the 512 columns of chunk wave + 4 i,
+  // the chunks of one row after those of the one before ----
+  const int chunks = (p.kp + 511) / 512;
+  Unit<T> v[Cfg::UNITS];
+  int unit_row[Cfg::UNITS], unit_col[Cfg::UNITS];
+#pragma unroll
+  for (int i = 0; i < Cfg::UNITS; ++i) {
+    unit_row[i] = (wave + 4 * i) / chunks;
+    unit_col[i] = (wave + 4 * i - unit_row[i] * chunks) * 512 + lane * 8;
+  }
+  auto load_rows = [&](int row0, int rows) {
+#pragma unroll
+    for (int i = 0; i < Cfg::UNITS; ++i) {
+      const int r = unit_row[i], col = unit_col[i];
+      if (r >= rows) break;
+      const int64_t src = kGather ? p.row_src[row0 + r] : row0 + r;
+      const T* const row = static_cast<const T*>(p.x) + src * p.k;
+      if (p.vec)
+        v[i].template load<true>(row, col, p.k);
+      else
+        v[i].template load<false>(row, col, p.k);
+    }
+  };
+  // (after a barrier behind the last reads of the tile before) the rows' codes and maxima
+  auto quantise = [&](int rows) {
+    if (threadIdx.x < Cfg::BM) s_top[threadIdx.x] = 0;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < Cfg::UNITS; ++i) {
+      const int r = unit_row[i];
+      if (r >= rows) break;
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, v[i].bits(j) & 0x7fffffffu);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+      if (lane == 0) atomicMax(&s_top[r], top);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < Cfg::UNITS; ++i) {
+      const int r = unit_row[i], col = unit_col[i];
+      if (r >= rows) break;
+      const uint32_t top = s_top[r];
+      const float most = __uint_as_float(top), shift = range_shift(most);
+      const C m = (C)most * (C)shift, inv = (C)127 / m;
+      const bool zero = top == 0 || top >= 0x7f800000u;
+      // 16-byte piece x of a step's 8 at piece x ^ (r & 7)
+      if (col < row_bytes) {
+        const int piece = (col >> 4 & 7) ^ (r & 7);
+        *reinterpret_cast<uint2*>(codes + r * row_bytes + (col & ~127) + piece * 16 + (col & 8)) =
+            zero ? make_uint2(0, 0) : v[i].template codes<C>(shift, m, inv);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+
+  const int frag_row = lane & 15, fq = lane >> 4, fsw = (frag_row >> 1) & 7;
+  int parity = 0, have = -1;
+  for (int unit = blockIdx.x; unit < total; unit += G) {
+    const int mt = unit / p.n_tiles_n, nt = unit - mt * p.n_tiles_n;
+    int e, row0, end;
+    p.tiles.get(mt, e, row0, end);
+    e = uniform(e), row0 = uniform(row0);
+    const int rows = min(Cfg::BM, uniform(end) - row0);
+    if (mt != have) {
+      load_rows(row0, rows);
+      if (have < 0)  // the first weights right behind the rows
+#pragma unroll 1
+        for (int i = 0; i < Cfg::STAGES; ++i)
+          if (l_live) issue();
+      quantise(rows);
+      have = mt;
+    }
+    const int my_row = min(frag_row, rows - 1);
+    const char* const ca = codes + my_row * row_bytes;
+    i32x4_t acc[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = i32x4_t{0, 0, 0, 0};
+    const int rot = n_steps > 0 ? (7 * e + 3 * nt) % n_steps : 0;
+    for (int step = 0; step < n_steps; ++step) {
+      int jr = step + rot;
+      if (jr >= n_steps) jr -= n_steps;
+      const int ks = wave + Cfg::WAVES * jr;
+      wait_groups<OPS, Cfg::STAGES - 1>(issued - used - 1);  // this step has landed
+      const char* sb = ring + (used % Cfg::STAGES) * Cfg::STAGE + frag_row * kRowBytes;
+      i32x4_t fa[2], fb[2][NC];
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh) {
+        const int chunk = kh * 4 + fq;
+        fa[kh] = *reinterpret_cast<const i32x4_t*>(ca + ks * kRowBytes + ((chunk ^ (my_row & 7)) << 4));
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          fb[kh][c] = *reinterpret_cast<const i32x4_t*>(sb + c * 16 * kRowBytes + ((chunk ^ fsw) << 4));
+      }
+      wait_lds();  // the stage has been read: it may be loaded again
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      ++used;
+      if (l_live) issue();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          acc[c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[kh][c], fa[kh], acc[c], 0, 0, 0);
+    }
+    constexpr int PIECES = Cfg::BN / 4, ROW = Cfg::BN * 4;
+    char* const red = smem + Cfg::RED_OFF + parity * (Cfg::WAVES * Cfg::RED_WAVE);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      *reinterpret_cast<i32x4_t*>(red + wave * Cfg::RED_WAVE + frag_row * ROW +
+                                  (((c * 4 + fq) ^ (frag_row & (PIECES - 1))) << 4)) = acc[c];
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    auto sum = [&](int r, int piece) {
+      i32x4_t t = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < Cfg::WAVES; ++w)
+        t += *reinterpret_cast<const i32x4_t*>(red + w * Cfg::RED_WAVE + r * ROW + ((piece ^ (r & (PIECES - 1))) << 4));
+      return t;
+    };
+    constexpr int CP = kGateUp ? PIECES / 2 : PIECES;  // pieces of output columns
+    const int r = threadIdx.x / CP, c = threadIdx.x % CP, n = nt * kCols + c * 4;
+    if (r < rows && n < p.n) {
+      const int64_t row = row0 + r;
+      const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      const f32x4_t s0 = four(p.s0, e, n, p.n), s1 = kGateUp ? four(p.s1, e, n, p.n) : zero;
+      const f32x4_t bias = !kGateUp && p.bias != nullptr ? bias_of<T>(p.bias, n, p.n) : zero;
+      const uint32_t top = s_top[r];
+      const float sa = top >= 0x7f800000u ? NAN : __uint_as_float(top) / 127.0f;
+      const i32x4_t g = sum(r, c);
+      const auto o = out_of<T, kGateUp>(g, kGateUp ? sum(r, CP + c) : g, sa, s0, s1, bias);
+      using E = std::conditional_t<std::is_same_v<T, bf16_t>, __bf16, T>;
+      E* const at = static_cast<E*>(p.c) + row * p.n + n;
+      if (p.n % 4 == 0) {
+        *reinterpret_cast<typename Out4<T>::type*>(at) = o;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < p.n) at[q] = o[q];
+      }
+    }
+    parity ^= 1;
+    // (the next tile's quantise() clears the maxima: not before these have been read)
+    if (unit + G < total && (unit + G) / p.n_tiles_n != mt) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+}
 #endif  // ASTRAI_MOE_RAGGED_K
 
 Args args_of(const Int8Gemm& g) {
@@ -957,6 +1187,8 @@ Args args_of(const Int8Gemm& g) {
   a.a = g.a, a.a_scale = g.a_scale, a.row_src = g.row_src;
   a.tiles = RowTiles{g.tiles, (int)g.n_rows, g.block_m};
   a.w0 = g.w0, a.w1 = g.w1, a.s0 = g.s0, a.s1 = g.s1, a.bias = g.bias;
+  a.x = g.x, a.k = g.k;
+  a.vec = g.k * (g.dtype == ASTRAI_MOE_BF16 ? 2 : 4) % 16 == 0 && aligned16(g.x);
   a.kp = (int)g.kp, a.n = (int)g.n, a.capacity = (int)g.capacity, a.c = g.c;
   return a;
 }
@@ -1053,12 +1285,38 @@ int launch_few(const Int8Gemm& g, hipStream_t s) {
     return launch_few_cfg<FewCfg<32, 16>, T, kGateUp, kGather>(g, s);
   return launch_few_cfg<FewCfg<32, 32>, T, kGateUp, kGather>(g, s);
 }
+
+template <typename T, bool kGateUp, bool kGather>
+int launch_quant(const Int8Gemm& g, hipStream_t s) {
+  if (g.capacity == 0) return ASTRAI_MOE_OK;
+  Args a = args_of(g);
+  const int64_t n_cols = ceil_div(g.n, kGateUp ? QuantCfg::BN / 2 : QuantCfg::BN);  // the last may be partial
+  a.n_tiles_n = (int)n_cols;
+  int64_t grid = 0;
+  if (int rc = persistent_grid(g.capacity, n_cols, &grid)) return rc;
+  hipLaunchKernelGGL((gemm_i8_quant_kernel<T, kGateUp, kGather>), dim3((unsigned)grid), dim3(QuantCfg::WAVES * 64), 0, s, a);
+  return check_launch(kGateUp ? "gemm_i8_quant_kernel<gate_up>" : "gemm_i8_quant_kernel<down>");
+}
 #endif
 
 }  // namespace
 
 #if ASTRAI_MOE_RAGGED_K
+// Where the registers and the LDS hold the rows, and a workgroup meets few row tiles,
+// each of which it quantises anew: one expert's rows, or at most two tiles a workgroup.
+bool int8_quantises(int64_t most_rows, int64_t k, int64_t row_tiles, int64_t n, bool gate_up) {
+  const int64_t tiles = row_tiles * ceil_div(n, gate_up ? QuantCfg::BN / 2 : QuantCfg::BN);
+  return (row_tiles == 1 || tiles <= 2 * cu_count()) && most_rows <= QuantCfg::BM &&
+         most_rows * ceil_div(k, 512) <= QuantCfg::WAVES * QuantCfg::UNITS;
+}
+
 namespace ragged {
+
+int launch_int8_quant(const Int8Gemm& g, hipStream_t s) {
+  if (g.dtype == ASTRAI_MOE_BF16)
+    return g.w1 != nullptr ? launch_quant<bf16_t, true, true>(g, s) : launch_quant<bf16_t, false, false>(g, s);
+  return g.w1 != nullptr ? launch_quant<float, true, true>(g, s) : launch_quant<float, false, false>(g, s);
+}
 
 int launch_int8_few(const Int8Gemm& g, hipStream_t s) {
   if (g.dtype == ASTRAI_MOE_BF16)
@@ -1070,6 +1328,7 @@ int launch_int8_few(const Int8Gemm& g, hipStream_t s) {
 
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s) {
 #if !ASTRAI_MOE_RAGGED_K
+  if (g.a == nullptr) return ragged::launch_int8_quant(g, s);
   if (aligned16(g.c) && few_rows(g.rows, g.block_m, g.kp / 2, g.n, g.w1 != nullptr)) return ragged::launch_int8_few(g, s);
   const int size = g.dtype == ASTRAI_MOE_BF16 ? 2 : 4;
   if (g.kp % kRowBytes != 0 || g.n * size % 16 != 0 || g.n % 4 != 0 || !aligned16(g.c))

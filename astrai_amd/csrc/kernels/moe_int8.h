@@ -19,8 +19,10 @@ constexpr int64_t kInt8MaxK = 131072;
 struct Int8Gemm {
   RowCounts rows;         // the rows as far as the host knows them
   int64_t a_bytes = 0;    // of a, where gathered
-  const int8_t* a;        // [*, kp]
+  const int8_t* a;        // [*, kp]; null: the kernel quantises the rows of x itself
   const float* a_scale;   // by row r
+  const void* x;          // [*, k] dtype
+  int64_t k;
   const int32_t* row_src;
   const int32_t* tiles;   // null: one expert's n_rows rows, in tiles of block_m
   int64_t capacity;       // tiles the list holds (without a list: ceil(n_rows / block_m))
@@ -58,6 +60,80 @@ __device__ __forceinline__ float swiglu<bf16_t>(int g, int u, float sa, float sg
 
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s);
 
+// round-half-even of 127 x / most, |x| <= most, exactly: n = the nearest integer to
+// the product with a rounded reciprocal is off by one at most, and the remainder 127
+// x - n most decides. C holds it exactly: 127 x and n most have 7 more bits than x
+// and most, and where n is not 0 their exponents are within 8 of each other (bf16
+// in 32 bits, fp32 in 64).
+template <typename C>
+__device__ __forceinline__ int code_of(C x, C most, C inv) {
+  C n = __builtin_elementwise_rint(x * inv);
+  const C d = __builtin_elementwise_fma(-n, most, x * (C)127), twice = (C)2 * __builtin_elementwise_abs(d);
+  const int i = (int)n;
+  const bool away = twice > most || (twice == most && (i & 1) != 0);
+  return away ? i + (d > (C)0 ? 1 : -1) : i;
+}
+
+template <typename T>
+struct CodeType {
+  typedef float type;  // of bf16
+};
+template <>
+struct CodeType<float> {
+  typedef double type;
+};
+
+// A power of two that brings a row's maximum away from the ends of the range, where
+// 127 x or 127 / most would leave it. (Values that vanish by it have code 0.)
+__device__ __forceinline__ float range_shift(float most) {
+  return most >= 0x1p100f ? 0x1p-64f : most < 0x1p-60f ? 0x1p64f : 1.0f;
+}
+
+__device__ __forceinline__ uint32_t word_of(bf16_t v) { return v; }
+__device__ __forceinline__ uint32_t word_of(float v) { return __float_as_uint(v); }
+
+// Eight consecutive values of a row in registers, two bf16 a word.
+template <typename T>
+struct Unit {
+  static constexpr int WORDS = 2 * sizeof(T);
+  uint32_t w[WORDS];
+  // from column c on, zeros from column k on; kVec: 16-byte loads (aligned rows)
+  template <bool kVec>
+  __device__ __forceinline__ void load(const T* row, int64_t c, int64_t k) {
+    if (kVec && c + 8 <= k) {
+#pragma unroll
+      for (int j = 0; j < WORDS; j += 4)
+        *reinterpret_cast<uint4*>(&w[j]) = *reinterpret_cast<const uint4*>(row + c + j * (4 / (int)sizeof(T)));
+    } else {
+      T in[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) in[j] = c + j < k ? row[c + j] : (T)0;
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j)
+        w[j] = sizeof(T) == 2 ? word_of(in[(2 * j) & 7]) | word_of(in[(2 * j + 1) & 7]) << 16 : word_of(in[j & 7]);
+    }
+  }
+  // the j-th value as a float's bits
+  __device__ __forceinline__ uint32_t bits(int j) const {
+    if constexpr (sizeof(T) == 2)
+      return (j & 1) != 0 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16;
+    else
+      return w[j];
+  }
+  // the codes for a row's shifted maximum `most`, 127 / most = inv
+  template <typename C>
+  __device__ __forceinline__ uint2 codes(float shift, C most, C inv) const {
+    union {
+      int8_t b[8];
+      uint2 u;
+    } o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o.b[j] = (int8_t)code_of<C>((C)__uint_as_float(bits(j)) * (C)shift, most, inv);
+    return o.u;
+  }
+};
+
+
 // On the matrix cores (moe_gemm_int8.hip); gate/up products are gathered (row_src),
 // the others not. a under 4 GiB where gathered. ragged: rows of a partial K step, or
 // outputs whose rows are no whole number of 16 bytes.
@@ -65,6 +141,10 @@ int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
 namespace ragged {
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
 int launch_int8_few(const Int8Gemm& g, hipStream_t s);  // few rows (few_rows), every shape; c aligned
+int launch_int8_quant(const Int8Gemm& g, hipStream_t s);
 }
+// Whether a product of row_tiles row tiles of at most most_rows rows of k values is to
+// quantise them itself (launch_int8_quant).
+bool int8_quantises(int64_t most_rows, int64_t k, int64_t row_tiles, int64_t n, bool gate_up);
 
 }  // namespace astrai_moe

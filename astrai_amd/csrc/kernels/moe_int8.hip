@@ -18,35 +18,6 @@
 namespace astrai_moe {
 namespace {
 
-// round-half-even of 127 x / most, |x| <= most, exactly: n = the nearest integer to
-// the product with a rounded reciprocal is off by one at most, and the remainder 127
-// x - n most decides. C holds it exactly: 127 x and n most have 7 more bits than x
-// and most, and where n is not 0 their exponents are within 8 of each other (bf16
-// in 32 bits, fp32 in 64).
-template <typename C>
-__device__ __forceinline__ int code_of(C x, C most, C inv) {
-  C n = __builtin_elementwise_rint(x * inv);
-  const C d = __builtin_elementwise_fma(-n, most, x * (C)127), twice = (C)2 * __builtin_elementwise_abs(d);
-  const int i = (int)n;
-  const bool away = twice > most || (twice == most && (i & 1) != 0);
-  return away ? i + (d > (C)0 ? 1 : -1) : i;
-}
-
-template <typename T>
-struct CodeType {
-  typedef float type;  // of bf16
-};
-template <>
-struct CodeType<float> {
-  typedef double type;
-};
-
-// A power of two that brings a row's maximum away from the ends of the range, where
-// 127 x or 127 / most would leave it. (Values that vanish by it have code 0.)
-__device__ __forceinline__ float range_shift(float most) {
-  return most >= 0x1p100f ? 0x1p-64f : most < 0x1p-60f ? 0x1p64f : 1.0f;
-}
-
 // Where a row's scale goes: scale[r], or the places of its token's rows in the
 // permuted order.
 struct ScaleOut {
@@ -61,9 +32,6 @@ struct ScaleOut {
     }
   }
 };
-
-__device__ __forceinline__ uint32_t word_of(bf16_t v) { return v; }
-__device__ __forceinline__ uint32_t word_of(float v) { return __float_as_uint(v); }
 
 // One row per WAVES waves, held in registers between its maximum and its codes: a
 // thread has NV units of 8 columns, WAVES * 512 columns apart. kVec: rows start on
@@ -82,34 +50,15 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   const T* const row = x + (on ? r : 0) * k;
   const int c0 = (WAVES == 1 ? lane : (int)threadIdx.x) * 8;
   if (clear != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *clear = 0;
-  constexpr int WORDS = 2 * sizeof(T);  // of a unit: values stay as they came, two bf16 a word
-  uint32_t v[NV][WORDS];
+  Unit<T> v[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = c0 + i * WAVES * 512;
-    if (kVec && c + 8 <= k && on) {
-#pragma unroll
-      for (int j = 0; j < WORDS; j += 4)
-        *reinterpret_cast<uint4*>(&v[i][j]) = *reinterpret_cast<const uint4*>(row + c + j * (4 / (int)sizeof(T)));
-    } else {
-      T in[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) in[j] = c + j < k && on ? row[c + j] : (T)0;
-#pragma unroll
-      for (int j = 0; j < WORDS; ++j)
-        v[i][j] = sizeof(T) == 2 ? (uint32_t)word_of(in[2 * j]) | (uint32_t)word_of(in[(2 * j + 1) & 7]) << 16 : word_of(in[j & 7]);
-    }
-  }
-  auto value = [&](int i, int j) {  // the unit's j-th value as a float's bits
-    if constexpr (sizeof(T) == 2) return (j & 1) != 0 ? v[i][j / 2] & 0xffff0000u : v[i][j / 2] << 16;
-    else return v[i][j];
-  };
+  for (int i = 0; i < NV; ++i) v[i].template load<kVec>(row, c0 + i * WAVES * 512, on ? k : 0);
   // (as integers, which order the magnitudes of floats, NaN above infinity)
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, value(i, j) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) top = max(top, v[i].bits(j) & 0x7fffffffu);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
   if constexpr (WAVES > 1) {
@@ -129,13 +78,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * WAVES * 512;
     if (c >= kp) continue;
-    union {
-      int8_t b[8];
-      uint2 u;
-    } o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o.b[j] = zero ? (int8_t)0 : (int8_t)code_of<C>((C)__uint_as_float(value(i, j)) * (C)shift, m, inv);
-    *reinterpret_cast<uint2*>(q + r * kp + c) = o.u;
+    *reinterpret_cast<uint2*>(q + r * kp + c) = zero ? make_uint2(0, 0) : v[i].template codes<C>(shift, m, inv);
   }
 }
 
@@ -389,6 +332,8 @@ int linear_block_m(int64_t n_rows, int64_t kp, int64_t n) {
   return n_rows < 96 ? kMfmaSmallBM : dense_gemm_block_m(n_rows, kp / 2, n, false);
 }
 
+bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 struct Parts {  // of a workspace, 256-byte aligned
   int64_t bytes = 0;
   int64_t take(int64_t n) {
@@ -440,6 +385,7 @@ RowCounts row_counts(const LayerSizes& z) { return {z.n_tokens * z.top_k, z.n_ex
 
 struct LayerPlan {
   int experts, slots, block_m;
+  bool quant_up, quant_down;  // the products quantise their rows themselves
   int64_t rows, tiles_len, dp, fp;
   int64_t topk_idx, topk_w, chunk_hist, chunk_base, offsets, sorted_token, sorted_w, token_pos, tiles, xq, xs, h, hq, hs,
       y, gemm_ws, gemm_ws_bytes = 0, bytes;
@@ -464,8 +410,14 @@ struct LayerPlan {
     tiles = p.take(tiles_len * 4);
     xq = p.take(T * dp);
     xs = p.take(rows * 4);  // by permuted row
-    // h is read once, to be quantised, before the down product writes y
-    h = y = p.take(rows * std::max(z.dim_ffn, z.dim) * size);
+    // h is read once, to be quantised, before the down product writes y (which a product
+    // that quantises it itself does meanwhile)
+    h = p.take(rows * std::max(z.dim_ffn, z.dim) * size);
+    // An expert meets a token once: its rows are at most the tokens.
+    const int64_t tiles_most = (tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE;
+    quant_up = int8_quantises(T, z.dim, tiles_most, z.dim_ffn, true);
+    quant_down = int8_quantises(T, z.dim_ffn, tiles_most, z.dim, false);
+    y = quant_down ? p.take(rows * z.dim * size) : h;
     hq = p.take(rows * fp);
     hs = p.take(rows * 4);
     if (block_m == kMfmaBigBM)
@@ -478,7 +430,7 @@ struct LayerPlan {
 }  // namespace
 
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s) {
-  if ((g.w1 != nullptr) == (g.row_src != nullptr) && (g.row_src == nullptr || g.a_bytes < (1ll << 32)))
+  if (g.a == nullptr || (g.w1 != nullptr) == (g.row_src != nullptr) && (g.row_src == nullptr || g.a_bytes < (1ll << 32)))
     return launch_int8_mfma(g, s);
   return g.dtype == ASTRAI_MOE_BF16 ? launch_general<bf16_t>(g, s) : launch_general<float>(g, s);
 }
@@ -487,7 +439,6 @@ int launch_int8_gemm(const Int8Gemm& g, hipStream_t s) {
 
 using namespace astrai_moe;
 
-static bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 extern "C" int64_t astrai_moe_int8_row_bytes(int64_t k) { return k < 0 ? -1 : int8_row_bytes(k); }
 
@@ -528,9 +479,14 @@ extern "C" int astrai_moe_int8_linear(const void* x, int dtype, const int8_t* w,
   int8_t* const q = reinterpret_cast<int8_t*>(base + p.q);
   float* const scale = reinterpret_cast<float*>(base + p.scale);
   int32_t* const claims = p.gemm_ws_bytes > 0 ? reinterpret_cast<int32_t*>(base + p.gemm_ws) : nullptr;
-  if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, claims, s)) return rc;
   Int8Gemm g{RowCounts(n_rows, 1)};
-  g.a = q, g.a_scale = scale, g.w0 = w, g.s0 = w_scale, g.bias = bias;
+  if (int8_quantises(n_rows, k, 1, n, false) && on16(out)) {
+    g.x = x, g.k = k;
+  } else {
+    if (int rc = launch_quantize_rows(x, dtype, n_rows, k, q, ScaleOut{scale, nullptr, 0}, claims, s)) return rc;
+    g.a = q, g.a_scale = scale;
+  }
+  g.w0 = w, g.s0 = w_scale, g.bias = bias;
   g.kp = int8_row_bytes(k), g.n = n, g.dtype = dtype, g.c = out;
   g.n_rows = n_rows, g.block_m = p.block_m, g.capacity = ceil_div(n_rows, g.block_m);
   if (p.gemm_ws_bytes > 0) g.ws = {base + p.gemm_ws, p.gemm_ws_bytes};
@@ -595,19 +551,30 @@ extern "C" int astrai_moe_int8_forward(const void* x, int dtype, const void* log
                                  nullptr, tiles, p.tiles_len, i32(p.chunk_base), stream)))
       return rc;
   }
-  if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq),
-                                 ScaleOut{f32(p.xs), i32(p.token_pos), p.slots}, claims, s))) return rc;
   Int8Gemm g{row_counts(z)};
   if (p.gemm_ws_bytes > 0) g.ws = {base + p.gemm_ws, p.gemm_ws_bytes};
-  g.a = i8(p.xq), g.a_scale = f32(p.xs), g.row_src = i32(p.sorted_token);
+  if (p.quant_up) {
+    g.x = x, g.k = dim;
+  } else {
+    if ((rc = launch_quantize_rows(x, dtype, n_tokens, dim, i8(p.xq), ScaleOut{f32(p.xs), i32(p.token_pos), p.slots},
+                                   claims, s)))
+      return rc;
+    g.a = i8(p.xq), g.a_scale = f32(p.xs), g.a_bytes = n_tokens * p.dp;
+  }
+  g.row_src = i32(p.sorted_token);
   g.tiles = tiles, g.capacity = (p.tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE;
   g.w0 = w_gate, g.w1 = w_up, g.s0 = gate_scale, g.s1 = up_scale;
-  g.a_bytes = n_tokens * p.dp;
   g.kp = p.dp, g.n = dim_ffn, g.dtype = dtype, g.c = base + p.h, g.block_m = p.block_m;
   if ((rc = launch_int8_gemm(g, s))) return rc;
-  if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq),
-                                 ScaleOut{f32(p.hs), nullptr, 0}, claims, s))) return rc;
-  g.a = i8(p.hq), g.a_scale = f32(p.hs), g.row_src = nullptr;
+  if (p.quant_down) {
+    g.a = nullptr, g.x = base + p.h, g.k = dim_ffn;
+  } else {
+    if ((rc = launch_quantize_rows(base + p.h, dtype, p.rows, dim_ffn, i8(p.hq), ScaleOut{f32(p.hs), nullptr, 0}, claims,
+                                   s)))
+      return rc;
+    g.a = i8(p.hq), g.a_scale = f32(p.hs);
+  }
+  g.row_src = nullptr;
   g.w0 = w_down, g.w1 = nullptr, g.s0 = down_scale, g.s1 = nullptr;
   g.kp = p.fp, g.n = dim, g.c = base + p.y;
   if ((rc = launch_int8_gemm(g, s))) return rc;
