@@ -115,15 +115,19 @@ extern "C" int64_t astrai_moe_forward_workspace_bytes(int64_t n_tokens, int n_ex
   return make_plan(z).bytes;
 }
 
-extern "C" int astrai_moe_forward(const void* x, const void* logits, const void* const* w_gate,
-                                  const void* const* w_up, const void* const* w_down, const void* const* packed_gate_up,
-                                  const void* const* packed_down, int dtype, int64_t n_tokens, int n_experts,
-                                  int top_k, int n_shared, int64_t dim, int64_t dim_ffn, void* workspace,
-                                  int64_t workspace_bytes, void* out, void* stream) {
+// routing: null (the reference's), or by scores of logits of logits_dtype.
+static int run_forward(const void* x, const void* logits, int logits_dtype, const float* bias,
+                       const astrai_moe_routing* routing, const void* const* w_gate, const void* const* w_up,
+                       const void* const* w_down, const void* const* packed_gate_up, const void* const* packed_down,
+                       int dtype, int64_t n_tokens, int n_experts, int top_k, int n_shared, int64_t dim,
+                       int64_t dim_ffn, void* workspace, int64_t workspace_bytes, void* out, void* stream) {
   clear_error();
   const Sizes z{n_tokens, n_experts, top_k, n_shared, dim, dim_ffn, dtype, packed_gate_up != nullptr};
   int rc = check_sizes(z);
   if (rc) return rc;
+  if (routing != nullptr &&
+      (rc = check_routing("forward", routing, logits_dtype, dtype, n_tokens, n_experts, top_k)))
+    return rc;
   if (n_tokens == 0) return ASTRAI_MOE_OK;
   ASTRAI_REQUIRE(x && logits && w_gate && w_up && w_down && workspace && out, "forward: null buffer");
   ASTRAI_REQUIRE((packed_gate_up == nullptr) == (packed_down == nullptr), "forward: one packed table without the other");
@@ -155,8 +159,14 @@ extern "C" int astrai_moe_forward(const void* x, const void* logits, const void*
   if (n_tokens <= ASTRAI_MOE_CHUNK_TOKENS && x_perm == nullptr) {
     const RouteList list{sorted_token, sorted_w, token_pos, tiles,
                          (p.tiles_len - ASTRAI_MOE_TILE_HEADER) / ASTRAI_MOE_TILE_STRIDE, p.block_m};
-    rc = launch_route_list(logits, dtype, n_tokens, n_experts, top_k, n_shared, list, s);
-  } else if ((rc = launch_route(logits, dtype, n_tokens, n_experts, top_k, n_shared, topk_idx, topk_w, hist, s)) == 0) {
+    rc = routing != nullptr ? launch_route_scores_list(logits, logits_dtype, bias, *routing, n_tokens, n_experts, top_k,
+                                                       n_shared, dtype, list, s)
+                            : launch_route_list(logits, dtype, n_tokens, n_experts, top_k, n_shared, list, s);
+  } else if ((rc = routing != nullptr
+                       ? launch_route_scores(logits, logits_dtype, bias, *routing, n_tokens, n_experts, top_k, n_shared,
+                                             dtype, topk_idx, topk_w, hist, s)
+                       : launch_route(logits, dtype, n_tokens, n_experts, top_k, n_shared, topk_idx, topk_w, hist, s)) ==
+             0) {
     rc = astrai_moe_permute(topk_idx, topk_w, hist, x, dtype, n_tokens, p.experts, p.slots, dim, p.block_m,
                             i32(p.offsets), sorted_token, sorted_w, token_pos, x_perm, tiles, p.tiles_len,
                             i32(p.chunk_base), stream);
@@ -180,6 +190,28 @@ extern "C" int astrai_moe_forward(const void* x, const void* logits, const void*
   const int64_t size = dtype == ASTRAI_MOE_BF16 ? 2 : 4;
   const void* shared = n_shared > 0 ? static_cast<const char*>(y) + n_tokens * top_k * dim * size : nullptr;
   return launch_combine(y, token_pos, nullptr, shared, n_shared, dtype, n_tokens, top_k, p.slots, dim, out, s);
+}
+
+extern "C" int astrai_moe_forward(const void* x, const void* logits, const void* const* w_gate,
+                                  const void* const* w_up, const void* const* w_down, const void* const* packed_gate_up,
+                                  const void* const* packed_down, int dtype, int64_t n_tokens, int n_experts,
+                                  int top_k, int n_shared, int64_t dim, int64_t dim_ffn, void* workspace,
+                                  int64_t workspace_bytes, void* out, void* stream) {
+  return run_forward(x, logits, dtype, nullptr, nullptr, w_gate, w_up, w_down, packed_gate_up, packed_down, dtype,
+                     n_tokens, n_experts, top_k, n_shared, dim, dim_ffn, workspace, workspace_bytes, out, stream);
+}
+
+extern "C" int astrai_moe_forward_scores(const void* x, const void* logits, int logits_dtype, const float* bias,
+                                         const astrai_moe_routing* routing, const void* const* w_gate,
+                                         const void* const* w_up, const void* const* w_down,
+                                         const void* const* packed_gate_up, const void* const* packed_down, int dtype,
+                                         int64_t n_tokens, int n_experts, int top_k, int n_shared, int64_t dim,
+                                         int64_t dim_ffn, void* workspace, int64_t workspace_bytes, void* out,
+                                         void* stream) {
+  clear_error();
+  ASTRAI_REQUIRE(routing != nullptr, "forward: null routing");
+  return run_forward(x, logits, logits_dtype, bias, routing, w_gate, w_up, w_down, packed_gate_up, packed_down, dtype,
+                     n_tokens, n_experts, top_k, n_shared, dim, dim_ffn, workspace, workspace_bytes, out, stream);
 }
 
 // One dense expert (MLP.forward, mlp.py:22-25) in one call. A decoding batch

@@ -93,6 +93,8 @@ _SIGNATURES: dict[str, tuple] = {
                                              _vp, _i64, _vp]),
     "astrai_moe_route_scores": (_int, [_vp, _int, _vp, _vp, _i64, _int, _int, _int, _vp, _vp, _vp, _vp]),
     "astrai_moe_route_scores_grad": (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _int, _int, _vp, _vp]),
+    "astrai_moe_forward_scores": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _int, _int, _int,
+                                         _i64, _i64, _vp, _i64, _vp, _vp]),
     "astrai_moe_expert_load": (_int, [_vp, _i64, _int, _vp, _vp]),
     "astrai_moe_balance_bias": (_int, [_vp, _vp, _int, _f32, _vp, _vp]),
     "astrai_moe_int8_row_bytes": (_i64, [_i64]),

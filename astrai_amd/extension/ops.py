@@ -509,16 +509,18 @@ def dense_block_m(n_tokens: int, dim: int, dim_ffn: int, dtype: torch.dtype) -> 
 
 def moe_routed_forward(x: torch.Tensor, logits: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                        w_down: torch.Tensor, dim_ffn: int, top_k: int,
-                       shared: torch.Tensor | None = None, packed: bool = False) -> torch.Tensor:
+                       shared: torch.Tensor | None = None, packed: bool = False, routing: Routing | None = None,
+                       bias: torch.Tensor | None = None) -> torch.Tensor:
     """Routed experts plus combine (mlp.py:84-100 and :71) for ``x [T, D]``
     given the router logits and the experts' weight-pointer tables (of packed
-    copies with ``packed``; ``w_up`` is then ignored)."""
+    copies with ``packed``; ``w_up`` is then ignored). ``routing`` (and
+    ``bias``): experts by scores, as ``moe_route_scores``."""
     n_tokens, dim = x.shape
     n_experts = logits.shape[1]
     if n_tokens == 0:
         return torch.empty(0, dim, dtype=x.dtype, device=x.device)
     block_m = select_block_m(n_tokens, n_experts, top_k, dim, dim_ffn, x.dtype)
-    route = moe_route(logits, top_k)
+    route = moe_route(logits, top_k) if routing is None else moe_route_scores(logits, top_k, routing, bias, x.dtype)
     if not packed and gather_supported(n_tokens, dim, dim_ffn, x.dtype):
         # the gate/up GEMM reads the token rows itself: no copied x_perm
         perm = moe_permute(route, x, n_experts, block_m, copy_rows=False)
@@ -556,21 +558,31 @@ def layer_forward_pays(n_tokens: int, n_shared: int, top_k: int, dim_ffn: int, i
 
 def moe_layer_forward(x: torch.Tensor, logits: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                       w_down: torch.Tensor, n_shared: int, dim_ffn: int, top_k: int,
-                      packed: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+                      packed: tuple[torch.Tensor, torch.Tensor] | None = None, routing: Routing | None = None,
+                      bias: torch.Tensor | None = None) -> torch.Tensor:
     """The layer's output for ``x [T, D]`` and its router logits (mlp.py:71-100)
     in one call of the library. The pointer tables hold the routed experts and
     then the ``n_shared`` shared ones; ``packed``: tables (gate/up, down) of
     their packed copies, read in place of the weights except by GEMMs of few
-    rows (the same bits)."""
+    rows (the same bits). ``routing`` (and ``bias``): experts by scores, as
+    ``moe_route_scores``."""
     _require_gpu(x, "x", 2)
     _require_gpu(logits, "logits", 2)
     code = _dtype_code(x, "x")
     n_tokens, dim = x.shape
     n_experts = logits.shape[1]
-    if logits.shape[0] != n_tokens or logits.dtype != x.dtype or logits.device != x.device:
+    if logits.shape[0] != n_tokens or (routing is None and logits.dtype != x.dtype) or logits.device != x.device:
         raise ValueError(f"logits must be [{n_tokens}, n_experts] {x.dtype} on {x.device}")
     if not 1 <= top_k <= n_experts:
         raise ValueError(f"top_k must be in [1, n_experts = {n_experts}], got {top_k}")
+    c_routing = None
+    if routing is not None:
+        c_routing = _check_routing(routing, n_experts, top_k)
+        logits_code = _dtype_code(logits, "logits")
+        if bias is not None:
+            _require_like(bias, "bias", (n_experts,), torch.float32, x)
+    elif bias is not None:
+        raise ValueError("a bias needs a routing by scores")
     tables = (w_gate, w_up, w_down, *(packed or ()))
     for name, t in zip(("w_gate", "w_up", "w_down", "packed gate/up", "packed down"), tables):
         _require_table(t, name, n_experts + n_shared, x)
@@ -581,6 +593,11 @@ def moe_layer_forward(x: torch.Tensor, logits: torch.Tensor, w_gate: torch.Tenso
     _check(0 if nbytes >= 0 else int(nbytes), "moe_layer_forward")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     pg, pd = (packed[0].data_ptr(), packed[1].data_ptr()) if packed is not None else (None, None)
+    if c_routing is not None:
+        _launch("astrai_moe_forward_scores", x, x.data_ptr(), logits.data_ptr(), logits_code, _ptr(bias),
+                ctypes.byref(c_routing), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), pg, pd, code, n_tokens,
+                n_experts, top_k, n_shared, dim, dim_ffn, ws.data_ptr(), nbytes, out.data_ptr())
+        return out
     _check(lib.astrai_moe_forward(x.data_ptr(), logits.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
                                   w_down.data_ptr(), pg, pd, code, n_tokens, n_experts, top_k, n_shared, dim, dim_ffn,
                                   ws.data_ptr(), nbytes, out.data_ptr(), _stream(x)), "moe_layer_forward")
@@ -804,21 +821,28 @@ def _check_routing(routing: Routing, n_experts: int, top_k: int) -> loader.CRout
 
 
 def _require_like(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, like: torch.Tensor) -> None:
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == like.device
+            and t.is_contiguous()):
+        return
     _require_gpu(t, name)
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {list(shape)} {dtype} on {like.device}, got {list(t.shape)} {t.dtype} on "
-                         f"{t.device}")
+    raise ValueError(f"{name} must be {list(shape)} {dtype} on {like.device}, got {list(t.shape)} {t.dtype} on "
+                     f"{t.device}")
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(name: str, like: torch.Tensor, *args) -> None:
     """Entry point ``name`` with ``like``'s device current and its current
     stream as the last argument."""
     fn = getattr(loader.library(), name)
-    if like.device.index == torch.cuda.current_device():
-        _check(fn(*args, _stream(like)), name)
+    if like.device.index == _current_device():
+        rc = fn(*args, _stream(like))
     else:
         with torch.cuda.device(like.device):
-            _check(fn(*args, _stream(like)), name)
+            rc = fn(*args, _stream(like))
+    if rc != 0:
+        _check(rc, name)
 
 
 def moe_route_scores(logits: torch.Tensor, top_k: int, routing: Routing = Routing(),

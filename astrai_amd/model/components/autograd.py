@@ -141,6 +141,30 @@ class RouteWeights(torch.autograd.Function):
         return ops.moe_route_grad(logits, topk_idx, dw.contiguous()), None
 
 
+class ScoredRouteWeights(torch.autograd.Function):
+    """Routing by scores with the weights' gradient back to the logits:
+    ``forward(logits [T, E], bias, top_k, routing, dtype)`` gives ``(topk_w,
+    topk_idx, chunk_hist)`` of ``ops.moe_route_scores``, differentiable in
+    ``logits`` through ``topk_w``. The bias moves the choice only."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, routing, dtype):
+        logits = logits.contiguous()
+        route = ops.moe_route_scores(logits, top_k, routing, bias, dtype)
+        ctx.routing = routing
+        ctx.save_for_backward(logits, route.topk_idx, route.topk_w)
+        ctx.mark_non_differentiable(route.topk_idx, route.chunk_hist)
+        return route.topk_w, route.topk_idx, route.chunk_hist
+
+    @staticmethod
+    def backward(ctx, dw, *_):
+        logits, topk_idx, topk_w = ctx.saved_tensors
+        if torch.is_grad_enabled():  # create_graph: the operators, whose gradient has one of its own
+            w = scored_weights(logits, topk_idx, topk_w, ctx.routing)
+            return (torch.autograd.grad(w, logits, dw, create_graph=True)[0], *[None] * 4)
+        return (ops.moe_route_scores_grad(logits, topk_idx, topk_w.detach(), dw.contiguous(), ctx.routing), *[None] * 4)
+
+
 class DenseExpert(torch.autograd.Function):
     """One dense SwiGLU expert (mlp.py:22-25, the shared experts and ``MLP``):
     ``forward(x [T, D], tables, dim_ffn, w_gate, w_up, w_down)``."""
@@ -191,3 +215,21 @@ def routing_weights(logits: Tensor, topk_idx: Tensor, dtype: torch.dtype) -> Ten
     probs = torch.softmax(logits.float(), dim=-1).to(dtype)
     w = probs.gather(1, topk_idx.long())
     return w / w.sum(dim=-1, keepdim=True)
+
+
+def scored_weights(logits: Tensor, topk_idx: Tensor, topk_w: Tensor, routing: ops.Routing) -> Tensor:
+    """The weights of ``ops.moe_route_scores`` at its choice as differentiable
+    torch ops, for derivatives of ``ScoredRouteWeights``' gradient (slots of
+    weight 0 have no part)."""
+    idx = topk_idx.long()
+    l = logits.float()
+    if routing.score == "sigmoid":
+        s = torch.sigmoid(l.gather(1, idx))
+    else:  # (a row whose experts are all off has no softmax)
+        off = torch.isinf(l).all(-1, keepdim=True)
+        s = torch.softmax(l.masked_fill(off, 0.0), dim=-1).gather(1, idx)
+    s = s.masked_fill(topk_w == 0, 0.0)
+    if routing.renormalise:
+        total = s.sum(-1, keepdim=True)
+        s = s / total.masked_fill(total == 0, 1.0)
+    return (s * routing.scale).to(topk_w.dtype)

@@ -280,6 +280,19 @@ class DeepSeekMoE(nn.Module):
         return (st.joint is not None and n_shared == self.n_shared_experts
                 and ops.layer_forward_supported(len(st.routed[0]), n_shared, self.n_activated_experts))
 
+    # -- routing (a layer that routes by scores overrides these) -------------------
+    def _routing(self) -> tuple[ops.Routing | None, Tensor | None]:
+        """The routing by scores and its bias; None, None: mlp.py:84-87."""
+        return None, None
+
+    def _route_autograd(self, logits: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+        """(weights in ``dtype``, experts, chunk histograms), the weights with
+        their gradient to the logits."""
+        if logits.dtype == dtype:
+            return RouteWeights.apply(logits, self.n_activated_experts)
+        topk_idx, _, chunk_hist = ops.moe_route(logits.detach(), self.n_activated_experts)
+        return routing_weights(logits, topk_idx, dtype), topk_idx, chunk_hist
+
     # -- forward ----------------------------------------------------------------
     def forward(self, x: Tensor) -> Tensor:
         bsz, seq_len, dim = x.shape
@@ -297,7 +310,7 @@ class DeepSeekMoE(nn.Module):
                 n_tokens, len(st.shared[0]), self.n_activated_experts, dim_ffn, x_flat.element_size()):
             packed = self._packed_tables(x_flat.dtype, st) if self.pack_weights else None
             out = ops.moe_layer_forward(x_flat, self.router(x_flat), *st.joint, len(st.shared[0]), dim_ffn,
-                                        self.n_activated_experts, packed)
+                                        self.n_activated_experts, packed, *self._routing())
         else:
             out = self._routed_forward(x_flat, st, self._shared_forward(x_flat, st))
         return out.view(bsz, seq_len, dim)
@@ -327,8 +340,8 @@ class DeepSeekMoE(nn.Module):
         else:
             tg, tu, td = st.tables[0]
         logits = self.router(x)
-        return ops.moe_routed_forward(x, logits, tg, tu, td, dim_ffn, self.n_activated_experts, shared,
-                                      packed=packed)
+        return ops.moe_routed_forward(x, logits, tg, tu, td, dim_ffn, self.n_activated_experts, shared, packed,
+                                      *self._routing())
 
     def _forward_autograd(self, x: Tensor, st: _ExpertState) -> Tensor:
         """mlp.py:64-100 with autograd: HIP kernels forward and backward.
@@ -343,12 +356,7 @@ class DeepSeekMoE(nn.Module):
         t_routed, t_shared = st.tables
         routed_w = st.routed
         dim_ffn = routed_w[0][0].shape[0]
-        logits = self.router(x)
-        if logits.dtype == x.dtype:
-            topk_w, topk_idx, chunk_hist = RouteWeights.apply(logits, self.n_activated_experts)
-        else:
-            topk_idx, _, chunk_hist = ops.moe_route(logits.detach(), self.n_activated_experts)
-            topk_w = routing_weights(logits, topk_idx, x.dtype)
+        topk_w, topk_idx, chunk_hist = self._route_autograd(self.router(x), x.dtype)
         routed = RoutedExperts.apply(x, topk_w, topk_idx, chunk_hist, t_routed, dim_ffn,
                                      *routed_w[0], *routed_w[1], *routed_w[2])
         if self.n_shared_experts == 0:

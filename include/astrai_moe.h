@@ -574,6 +574,24 @@ int astrai_moe_route_scores_grad(const void* logits, int dtype,
                                  int64_t n_tokens, int n_experts, int top_k,
                                  void* dlogits, void* stream);
 
+/*
+ * astrai_moe_forward with experts chosen by astrai_moe_route_scores (bias and
+ * routing as there; logits of logits_dtype, weights of dtype). The same
+ * workspace and limits.
+ */
+int astrai_moe_forward_scores(const void* x, const void* logits,
+                              int logits_dtype, const float* bias,
+                              const astrai_moe_routing* routing,
+                              const void* const* w_gate,
+                              const void* const* w_up,
+                              const void* const* w_down,
+                              const void* const* packed_gate_up,
+                              const void* const* packed_down, int dtype,
+                              int64_t n_tokens, int n_experts, int top_k,
+                              int n_shared, int64_t dim, int64_t dim_ffn,
+                              void* workspace, int64_t workspace_bytes,
+                              void* out, void* stream);
+
 /* load[e]: tokens routed to expert e, from the chunks' histograms [n_chunks, n_experts]. */
 int astrai_moe_expert_load(const int32_t* chunk_hist, int64_t n_chunks,
                            int n_experts, int32_t* load, void* stream);

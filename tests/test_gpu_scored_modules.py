@@ -1,0 +1,305 @@
+"""The modules around the operators: ``ScoredMoE`` (inference and training),
+``Int8Linear`` and ``Int8MoE``, against plain 64-bit layers at the kernels'
+choice of experts, which test_gpu_route_scores.py compares by itself.
+
+Tolerances, of the norm: fp32 layers sum K <= 1024 products in 32 bits, off by at
+most K 2^-24 = 2^-14 of them. bf16 layers round h, y, each weight and every add of
+the combine (top_k + 1 of them), each by 2^-8 at most, and their gradients dy, dh,
+dg, du and dx on the way: sqrt(12) 2^-8 < 2e-2 for independent roundings.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from astrai_amd.extension import ops
+from astrai_amd.model.components.int8 import Int8Linear, Int8MoE, quantize_moe
+from astrai_amd.model.components.linear import Linear
+from astrai_amd.model.components.mlp import MLP, DeepSeekMoE, FFNFactory
+from astrai_amd.model.components.scored_moe import ScoredMoE
+from oracle import operators_ref as R
+
+pytestmark = pytest.mark.gpu
+
+REL = {torch.bfloat16: 2e-2, torch.float32: 2.0 ** -14}
+GROUPED = dict(score_func="sigmoid", n_groups=4, topk_groups=2, group_top=2, route_scale=2.5)
+
+
+def _layer(gpu, dtype, dim=256, dim_ffn=192, experts=16, shared=1, top_k=4, seed=0, cls=ScoredMoE, **routing):
+    torch.manual_seed(seed)
+    layer = cls(dim, dim_ffn, experts, shared, top_k, **routing)
+    for m in layer.modules():
+        if hasattr(m, "reset_parameters"):
+            m.reset_parameters()
+    with torch.no_grad():
+        layer.router.weight.normal_(0.0, 0.1)
+        for n, p in layer.named_parameters():
+            if "router" not in n:
+                p.normal_(0.0, 0.06)
+        if cls is ScoredMoE:
+            layer.balance_bias.normal_(0.0, 0.05)
+    return layer.to(device=gpu, dtype=dtype)
+
+
+def _plain(layer, x, leaves):
+    """The layer in float64 from float64 leaves (name -> tensor), at the choice
+    that its own logits give."""
+    logits = layer.router(x.detach())
+    route = ops.moe_route_scores(logits, layer.n_activated_experts, layer.routing, layer.balance_bias, x.dtype)
+    chosen, live = route.topk_idx.long(), route.topk_w != 0
+    l64 = leaves["x"] @ leaves["router.weight"].t()
+    l64 = l64 + (logits.double() - l64).detach()  # the values as the layer rounds them, their gradient as is
+    s = torch.sigmoid(l64) if layer.routing.score == "sigmoid" else torch.softmax(l64, -1)
+    w = R.weights(s, chosen, live, layer.routing)
+
+    def mlp(prefix, rows):
+        g, u, d = (leaves[f"{prefix}.{n}.weight"] for n in ("gate", "up", "down"))
+        return (torch.nn.functional.silu(rows @ g.t()) * (rows @ u.t())) @ d.t()
+
+    out = torch.zeros_like(leaves["x"])
+    for i in range(layer.n_shared_experts):
+        out = out + mlp(f"shared_experts.{i}", leaves["x"]) / layer.n_shared_experts
+    for e in range(layer.n_routed_experts):
+        token, slot = (chosen == e).nonzero(as_tuple=True)
+        if token.numel():
+            out = out.index_add(0, token, mlp(f"routed_experts.{e}", leaves["x"][token]) * w[token, slot].unsqueeze(1))
+    return out
+
+
+def _leaves(layer, x, grad=False):
+    got = {n: p.detach().double().requires_grad_(grad) for n, p in layer.named_parameters()}
+    got["x"] = x.detach().double().requires_grad_(grad)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens", [1, 20, 33, 300])
+@pytest.mark.parametrize("shared,routing", [(1, GROUPED), (0, dict(score_func="softmax", renormalise=False, route_scale=4.0)),
+                                            (2, dict(score_func="softmax", n_groups=8, topk_groups=3))])
+def test_inference(gpu, dtype, tokens, shared, routing):
+    layer = _layer(gpu, dtype, shared=shared, **routing).requires_grad_(False)
+    x = torch.randn(1, tokens, 256, device=gpu).to(dtype)
+    want = _plain(layer, x[0], _leaves(layer, x[0]))
+    got = layer(x)
+    assert got.shape == x.shape and got.dtype == dtype
+    assert (got[0].double() - want).norm() <= REL[dtype] * want.norm()
+    # the separate calls of the pipeline (as many shared rows take) give the same layer
+    st = layer._current(dtype, x.device)
+    apart = layer._routed_forward(x[0], st, layer._shared_forward(x[0], st))
+    assert (apart.double() - want).norm() <= REL[dtype] * want.norm()
+
+
+def test_default_routing_is_the_reference_layer(gpu):
+    """Softmax, renormalised, no groups, no bias, fp32: DeepSeekMoE's layer."""
+    scored = _layer(gpu, torch.float32)
+    scored.balance_bias.zero_()
+    ref = _layer(gpu, torch.float32, cls=DeepSeekMoE)
+    ref.load_state_dict({k: v for k, v in scored.state_dict().items() if k != "balance_bias"})
+    x = torch.randn(2, 40, 256, device=gpu)
+    with torch.no_grad():
+        a, b = scored(x), ref(x)
+    assert (a - b).norm() <= 2.0 ** -16 * b.norm()  # weights: 70 * 2^-24 each way, then the same kernels
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("routing", [GROUPED, dict(score_func="softmax", renormalise=False, route_scale=4.0)])
+def test_training(gpu, dtype, routing):
+    layer = _layer(gpu, dtype, **routing)
+    x = torch.randn(1, 200, 256, device=gpu).to(dtype).requires_grad_(True)
+    dout = torch.randn(1, 200, 256, device=gpu).to(dtype)
+    leaves = _leaves(layer, x[0], grad=True)
+    want = _plain(layer, x[0], leaves)
+    want.backward(dout[0].double())
+    out = layer(x)
+    out.backward(dout)
+    assert (out[0].double() - want).norm() <= REL[dtype] * want.norm()
+    for name, p in (*layer.named_parameters(), ("x", x)):
+        ref = leaves[name].grad
+        got = p.grad.view(ref.shape).double()
+        assert (got - ref).norm() <= 2 * REL[dtype] * ref.norm(), name
+    assert layer.balance_bias.grad is None
+
+
+def test_second_derivatives_reach_the_logits(gpu):
+    """The weights' gradient with create_graph, and its gradient, against the
+    plain weights' (float32: 70 roundings, twice)."""
+    from astrai_amd.model.components.autograd import ScoredRouteWeights
+
+    for routing in (ops.Routing("sigmoid", scale=2.0), ops.Routing("softmax", renormalise=False)):
+        logits = torch.randn(24, 16, device=gpu, requires_grad=True)
+        v, u = torch.randn(24, 4, device=gpu), torch.randn(24, 16, device=gpu)
+        w, idx, _ = ScoredRouteWeights.apply(logits, None, 4, routing, torch.float32)
+        (g,) = torch.autograd.grad(w, logits, v, create_graph=True)
+        (gg,) = torch.autograd.grad(g, logits, u)
+        l64 = logits.detach().double().requires_grad_(True)
+        s = torch.sigmoid(l64) if routing.score == "sigmoid" else torch.softmax(l64, -1)
+        w64 = R.weights(s, idx.long(), torch.ones_like(idx, dtype=torch.bool), routing)
+        (g64,) = torch.autograd.grad(w64, l64, v.double(), create_graph=True)
+        (gg64,) = torch.autograd.grad(g64, l64, u.double())
+        assert (g.double() - g64).norm() <= 2.0 ** -16 * g64.norm()
+        assert (gg.double() - gg64).norm() <= 2.0 ** -16 * gg64.norm()
+
+
+def test_balance_over_training_steps(gpu):
+    """Tracked loads add up over forwards; the update moves the bias by the rate
+    against them and starts over; without tracked forwards nothing changes."""
+    layer = _layer(gpu, torch.float32, track_load=True, **GROUPED)
+    before = layer.balance_bias.clone()
+    want = torch.zeros(16, dtype=torch.int64, device=gpu)
+    for seed in range(3):
+        x = torch.randn(1, 50, 256, device=gpu, generator=torch.Generator("cuda").manual_seed(seed))
+        idx = ops.moe_route_scores(layer.router(x[0]).detach(), 4, layer.routing, layer.balance_bias).topk_idx
+        want += torch.bincount(idx.long().view(-1), minlength=16)
+        layer(x)
+    layer.eval()
+    layer(x)  # evaluation is not counted
+    layer.train()
+    load = layer.update_balance(0.01)
+    assert torch.equal(load.long(), want)
+    step = torch.sign((want.sum() - 16 * want).double()) * 0.01
+    assert ((layer.balance_bias.double() - before.double() - step).abs() <= 2.0 ** -24 * (before.abs() + 0.02)).all()
+    after = layer.balance_bias.clone()
+    assert layer.update_balance(0.01) is None and torch.equal(layer.balance_bias, after)
+
+
+def test_balance_bias_keeps_its_32_bits(gpu):
+    layer = _layer(gpu, torch.float32, **GROUPED)
+    bias = layer.balance_bias.clone()
+    layer.to(torch.bfloat16)
+    assert layer.balance_bias.dtype == torch.float32 and torch.equal(layer.balance_bias, bias)
+    assert layer.router.weight.dtype == torch.bfloat16
+    other = ScoredMoE(256, 192, 16, 1, 4, **GROUPED).to(device=gpu, dtype=torch.bfloat16)
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other.balance_bias, bias)
+
+
+def test_no_tokens_and_refusals(gpu):
+    layer = _layer(gpu, torch.bfloat16, **GROUPED)
+    with torch.no_grad():
+        assert layer(torch.empty(1, 0, 256, dtype=torch.bfloat16, device=gpu)).shape == (1, 0, 256)
+    assert FFNFactory.get_component_class("moe_scored") is ScoredMoE
+    for bad in (dict(score_func="tanh"), dict(n_groups=3), dict(n_groups=4, topk_groups=5),
+                dict(n_groups=16, topk_groups=2)):
+        with pytest.raises(ValueError):
+            ScoredMoE(64, 64, 16, 1, 4, **bad)
+    int8 = Int8MoE.from_layer(layer)
+    x = torch.randn(1, 3, 256, device=gpu).bfloat16().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference"):
+        int8(x)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        int8(torch.randn(1, 3, 256))
+    assert int8(torch.empty(1, 0, 256, dtype=torch.bfloat16, device=gpu)).shape == (1, 0, 256)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["scored", "reference"])
+@pytest.mark.parametrize("tokens", [1, 30, 200])
+def test_int8_layer_from_a_float_layer(gpu, dtype, kind, tokens):
+    """Int8MoE is moe_int8_forward on the layer's quantised weights, and its
+    output the layer's up to the codes: each of the three products is off by two
+    roundings to 127 steps of at most 8 rms, 2 * (8 / 127) / sqrt(12) = 3.6e-2 of
+    its norm, together below 7e-2."""
+    layer = _layer(gpu, dtype, cls=ScoredMoE if kind == "scored" else DeepSeekMoE, **(GROUPED if kind == "scored" else {}))
+    layer.requires_grad_(False).eval()
+    int8 = Int8MoE.from_layer(layer)
+    x = torch.randn(1, tokens, 256, device=gpu).to(dtype)
+    got, base = int8(x), layer(x)
+    logits = layer.router(x[0])
+    routing, bias = layer._routing()
+    assert torch.equal(got[0], ops.moe_int8_forward(x[0], logits, int8.experts(), 4, 1, routing, bias))
+    assert (got.double() - base.double()).norm() <= 7e-2 * base.double().norm()
+    # through a state dict into an empty module
+    again = Int8MoE(256, 192, 16, 1, 4, routing).to(device=gpu, dtype=dtype)
+    again.load_state_dict(int8.state_dict())
+    assert torch.equal(again(x), got)
+
+
+def test_int8_scales_keep_their_32_bits(gpu):
+    layer = _layer(gpu, torch.float32, **GROUPED).requires_grad_(False)
+    int8 = Int8MoE.from_layer(layer)
+    scales = {n: int8._buffers[n].clone() for n in Int8MoE.SCALES}
+    int8.to(torch.bfloat16)
+    for n, s in scales.items():
+        assert int8._buffers[n].dtype == torch.float32 and torch.equal(int8._buffers[n], s)
+    lin = Linear(64, 32, bias=True)
+    lin.reset_parameters()  # (allocated, not initialised, by the constructor)
+    lin = Int8Linear.from_linear(lin.to(gpu))
+    s = lin.weight_scale.clone()
+    lin.to(torch.bfloat16)
+    assert lin.weight_scale.dtype == torch.float32 and torch.equal(lin.weight_scale, s)
+    assert lin.weight.dtype == torch.int8 and lin.bias.dtype == torch.bfloat16
+
+
+def test_int8_linear_module(gpu):
+    torch.manual_seed(0)
+    lin = Linear(100, 72, bias=True)
+    lin.reset_parameters()
+    lin = lin.to(gpu)
+    int8 = Int8Linear.from_linear(lin)
+    x = torch.randn(2, 3, 100, device=gpu)
+    got = int8(x)
+    assert got.shape == (2, 3, 72)
+    want = R.int8_linear(x.view(6, 100), int8.weight, int8.weight_scale, lin.bias)
+    assert (got.view(6, 72).double() - want).abs().max() <= 2.0 ** -20 * want.abs().max()
+    again = Int8Linear(100, 72, bias=True).to(gpu)
+    again.load_state_dict(int8.state_dict())
+    assert torch.equal(again(x), got)
+
+
+def test_quantize_moe_inside_a_model(gpu):
+    class Block(torch.nn.Module):
+        def __init__(self, ffn):
+            super().__init__()
+            self.mlp, self.dense = ffn, MLP(256, 192)
+
+        def forward(self, x):
+            return self.mlp(x) + x
+
+    model = torch.nn.Sequential(Block(_layer(gpu, torch.bfloat16, **GROUPED)),
+                                Block(_layer(gpu, torch.bfloat16, cls=DeepSeekMoE))).requires_grad_(False)
+    x = torch.randn(1, 16, 256, device=gpu).bfloat16()
+    base = model(x)
+    assert quantize_moe(model) == 2
+    assert all(isinstance(b.mlp, Int8MoE) and isinstance(b.dense, MLP) for b in model)
+    assert (model(x).double() - base.double()).norm() <= 7e-2 * base.double().norm()
+
+
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_captured_layers_replay(gpu, tokens):
+    """A scored layer and its int8 form captured together: every replay equals
+    the eager calls, on refilled inputs, with eager work between."""
+    layer = _layer(gpu, torch.bfloat16, **GROUPED).requires_grad_(False)
+    int8 = Int8MoE.from_layer(layer)
+    x = torch.randn(1, tokens, 256, device=gpu).bfloat16()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        int8(layer(x))
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            a = layer(x)
+            b = int8(a)
+    torch.cuda.current_stream().wait_stream(stream)
+    for i in range(4):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).bfloat16())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, layer(x)) and torch.equal(b, int8(a))
+
+
+def test_balance_sums_over_a_gloo_group(gpu):
+    import torch.distributed as dist
+
+    store = dist.HashStore()
+    dist.init_process_group("gloo", store=store, rank=0, world_size=1)
+    try:
+        layer = _layer(gpu, torch.float32, track_load=True, **GROUPED)
+        layer(torch.randn(1, 50, 256, device=gpu))
+        load = layer.update_balance(0.01, group=dist.group.WORLD)
+        assert load.sum().item() == 200
+    finally:
+        dist.destroy_process_group()
