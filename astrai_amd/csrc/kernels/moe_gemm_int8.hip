@@ -1310,6 +1310,29 @@ bool int8_quantises(int64_t most_rows, int64_t k, int64_t row_tiles, int64_t n, 
          most_rows * ceil_div(k, 512) <= QuantCfg::WAVES * QuantCfg::UNITS;
 }
 
+// Where the few-row kernels replace the tiles of 64 or 128 rows: as few_rows says of
+// the bf16 ones, but for more than 32 rows of one expert only where a round holds all
+// the column tiles, each of which stages every row again (us a product with / without
+// them: 4096 to 14336, 448 tiles, 40 rows 31.9 / 25.5, 100 38.2 / 26.4; 14336 to 4096,
+// 128 tiles, 40 25.5 / 63.5, 128 34.7 / 64.7; 2048 to 5632, 176 tiles, 64 11.5 / 14.6).
+// And routed rows of short products only where two rounds hold their column tiles:
+// with fewer than kFewMinSteps K steps, of which a wave takes every fourth, a tile's
+// sums cost more than its loads (us a layer with / without: 64 experts, top-6 and a
+// shared one, D 2048, F 1408, 2 tokens 49.4 / 42.6, 8 95 / 84; 128 experts, top-8, D
+// 4096, F 1536, 16 335 / 300; long ones gain: 8 experts, D 4096, F 14336, 2 tokens 132 /
+// 175, 32 275 / 297).
+constexpr int kFewMinSteps = 20;
+bool int8_few_rows(const RowCounts& rows, int block_m, int64_t kp, int64_t n, bool gate_up) {
+  const double cols = (double)ceil_div(n, gate_up ? 16 : 32);
+  if (rows.dense()) {
+    if (rows.exact_rows > 32 && cols > cu_count()) return false;
+  } else if (ceil_div(kp, kRowBytes) < kFewMinSteps) {
+    const double e = rows.experts, live = e > 0 ? e * (1.0 - std::pow(1.0 - 1.0 / e, (double)rows.rows)) : 0.0;
+    if ((live + rows.exact) * cols > 2.0 * cu_count()) return false;
+  }
+  return few_rows(rows, block_m, kp / 2, n, gate_up);
+}
+
 namespace ragged {
 
 int launch_int8_quant(const Int8Gemm& g, hipStream_t s) {
@@ -1329,7 +1352,7 @@ int launch_int8_few(const Int8Gemm& g, hipStream_t s) {
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s) {
 #if !ASTRAI_MOE_RAGGED_K
   if (g.a == nullptr) return ragged::launch_int8_quant(g, s);
-  if (aligned16(g.c) && few_rows(g.rows, g.block_m, g.kp / 2, g.n, g.w1 != nullptr)) return ragged::launch_int8_few(g, s);
+  if (aligned16(g.c) && int8_few_rows(g.rows, g.block_m, g.kp, g.n, g.w1 != nullptr)) return ragged::launch_int8_few(g, s);
   const int size = g.dtype == ASTRAI_MOE_BF16 ? 2 : 4;
   if (g.kp % kRowBytes != 0 || g.n * size % 16 != 0 || g.n % 4 != 0 || !aligned16(g.c))
     return ragged::launch_int8_mfma(g, s);

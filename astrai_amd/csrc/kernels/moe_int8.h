@@ -140,9 +140,11 @@ struct Unit {
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
 namespace ragged {
 int launch_int8_mfma(const Int8Gemm& g, hipStream_t s);
-int launch_int8_few(const Int8Gemm& g, hipStream_t s);  // few rows (few_rows), every shape; c aligned
+int launch_int8_few(const Int8Gemm& g, hipStream_t s);  // few rows, every shape; c aligned
 int launch_int8_quant(const Int8Gemm& g, hipStream_t s);
 }
+// Whether a product runs on the few-row kernels.
+bool int8_few_rows(const RowCounts& rows, int block_m, int64_t kp, int64_t n, bool gate_up);
 // Whether a product of row_tiles row tiles of at most most_rows rows of k values is to
 // quantise them itself (launch_int8_quant).
 bool int8_quantises(int64_t most_rows, int64_t k, int64_t row_tiles, int64_t n, bool gate_up);

@@ -329,7 +329,9 @@ int layer_block_m(int64_t rows_per_expert) {
                                  : kMfmaBigBM;
 }
 int linear_block_m(int64_t n_rows, int64_t kp, int64_t n) {
-  return n_rows < 96 ? kMfmaSmallBM : dense_gemm_block_m(n_rows, kp / 2, n, false);
+  if (n_rows <= 32 || (n_rows < 96 && int8_few_rows(RowCounts(n_rows, 1), kMfmaSmallBM, kp, n, false)))
+    return kMfmaSmallBM;
+  return dense_gemm_block_m(n_rows, kp / 2, n, false);
 }
 
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
