@@ -191,7 +191,7 @@ __device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16
   const int n_base = kGateUp ? t_nt * (BN / 2) + wn * (WN / 2) : t_nt * BN + wn * WN;
   const int N = p.n;
   T* const C = static_cast<T*>(p.c);
-  const bool whole = !kRagged || (N * (int)sizeof(T)) % 16 == 0;
+  const bool whole = !kRagged || ((N * (int)sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0);
 #pragma unroll
   for (int jp = 0; jp < NJ; jp += 2) {
     f32x4_t s0[2], s1[2], b[2];

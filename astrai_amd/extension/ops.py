@@ -845,6 +845,25 @@ def _launch(name: str, like: torch.Tensor, *args) -> None:
         _check(rc, name)
 
 
+def _bytes(name: str, like: torch.Tensor, *args) -> int:
+    """Workspace bytes of an entry point on ``like``'s device."""
+    fn = getattr(loader.library(), name)
+    if like.device.index == _current_device():
+        n = fn(*args)
+    else:
+        with torch.cuda.device(like.device):
+            n = fn(*args)
+    if n < 0:
+        _check(int(n), name)
+    return n
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
+            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
 def moe_route_scores(logits: torch.Tensor, top_k: int, routing: Routing = Routing(),
                      bias: torch.Tensor | None = None, weight_dtype: torch.dtype | None = None) -> RouteResult:
     """Experts by softmax or sigmoid scores, with a bias for balance (float,
@@ -978,9 +997,10 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
     _require_like(w_scale, "w_scale", (n,), torch.float32, x)
     if bias is not None:
         _require_like(bias, "bias", (n,), x.dtype, x)
+    if out is not None and _overlap(out, x):
+        raise ValueError("out must not overlap x")
     out = _out_buffer(out, m, n, x)
-    nbytes = loader.library().astrai_moe_int8_linear_workspace_bytes(m, k, n, code)
-    _check(0 if nbytes >= 0 else int(nbytes), "int8_linear")
+    nbytes = _bytes("astrai_moe_int8_linear_workspace_bytes", x, m, k, n, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _launch("astrai_moe_int8_linear", x, x.data_ptr(), code, w.data_ptr(), w_scale.data_ptr(), _ptr(bias), m, k, n,
             ws.data_ptr(), nbytes, out.data_ptr())
@@ -1032,9 +1052,7 @@ def moe_int8_forward(x: torch.Tensor, logits: torch.Tensor, experts: Int8Experts
         _require_codes(getattr(experts, name), name, (e, n, int8_row_bytes(k)), x)
         _require_like(getattr(experts, name + "_scale"), name + "_scale", (e, n), torch.float32, x)
     out = torch.empty_like(x)
-    nbytes = loader.library().astrai_moe_int8_forward_workspace_bytes(n_tokens, n_experts, top_k, n_shared, dim, dim_ffn,
-                                                                      code)
-    _check(0 if nbytes >= 0 else int(nbytes), "moe_int8_forward")
+    nbytes = _bytes("astrai_moe_int8_forward_workspace_bytes", x, n_tokens, n_experts, top_k, n_shared, dim, dim_ffn, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _launch("astrai_moe_int8_forward", x, x.data_ptr(), code, logits.data_ptr(), logits_code, _ptr(bias), c_routing,
             experts.gate.data_ptr(), experts.up.data_ptr(), experts.down.data_ptr(), experts.gate_scale.data_ptr(),

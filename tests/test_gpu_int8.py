@@ -172,6 +172,28 @@ def test_out_is_written_where_it_belongs(gpu, m, k, n):
     assert (buf[0] == 7).all() and (buf[m + 1] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 512, 520), (20, 640, 264), (70, 1000, 264), (600, 512, 1032), (300, 512, 1000)])
+def test_operands_off_16_byte_boundaries(gpu, m, k, n, dtype):
+    """x, out, bias and scales that start one value behind a boundary: the same
+    bits as aligned ones, and no neighbour of out written."""
+    def shifted(t, fill=0.0):
+        buf = torch.full((t.numel() + 2,), fill, dtype=t.dtype, device=gpu)
+        buf[1:-1] = t.reshape(-1)
+        return buf, buf[1:-1].view(t.shape)
+
+    x = _randn(gpu, m, k, dtype=dtype)
+    w, ws = _weight(gpu, n, k, 2)
+    bias = _randn(gpu, n, seed=3, dtype=dtype)
+    want = ops.int8_linear(x, w, ws, bias)
+    buf, out = shifted(torch.zeros_like(want), 7.0)
+    got = ops.int8_linear(shifted(x)[1], w, shifted(ws)[1], shifted(bias)[1], out=out)
+    assert torch.equal(got, want) and buf[0] == 7.0 and buf[-1] == 7.0
+    q, s = ops.quantize_rows(shifted(x)[1])
+    want_q, want_s = ops.quantize_rows(x)
+    assert torch.equal(q, want_q) and torch.equal(s, want_s)
+
+
 def test_rows_do_not_depend_on_their_company(gpu):
     """Exact sums: a row's bits are the same in every batch, whatever kernel its
     size takes."""
@@ -343,6 +365,9 @@ def test_int8_refusals(gpu):
     for args in bad:
         with pytest.raises(ValueError):
             ops.int8_linear(*args)
+    square, sq = _weight(gpu, 64, 64, 0)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.int8_linear(x, square, sq, out=x)
     with pytest.raises(ValueError, match="out must be"):
         ops.int8_linear(x, w, ws, out=torch.empty(4, 23, dtype=torch.bfloat16, device=gpu))
     experts = _experts(gpu, 5, 64, 96)
