@@ -297,7 +297,7 @@ __device__ __forceinline__ uint64_t groups_kept(const F (&value)[C], float tol, 
     last = lanes_max<L>(mine);
     // (groups without live experts: the lowest not kept yet)
     const int at = last > kOffKey ? first_lane<L>(mine == last) / p : __builtin_ctzll(~kept);
-    kept |= 1ull << at;
+    kept |= 1ull << (at & 63);
     if (g == at) mine = kOffKey;
   }
   if (tol > 0.0f) close = near((float)last, (float)lanes_max<L>(mine), 2.0f * tol);
@@ -310,7 +310,7 @@ __device__ __forceinline__ void in_kept(uint64_t kept, int sub, int per, bool (&
   int g = sub * C / per, left = per - (sub * C - g * per);
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    in[i] = (kept >> g & 1) != 0;
+    in[i] = (kept >> (g & 63) & 1) != 0;
     if (--left == 0) left = per, ++g;
   }
 }
@@ -499,7 +499,7 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
     bool close = false, in[C];
     uint64_t kept = 0;
     if constexpr (kGroups) {
-      kept = groups_kept<L, C>(value, tol, sub, opt, n_experts, m, close);
+      if (opt.n_groups <= L) kept = groups_kept<L, C>(value, tol, sub, opt, n_experts, m, close);
       in_kept<C>(kept, sub, n_experts / opt.n_groups, in);
     }
 #pragma unroll
@@ -527,7 +527,7 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
                      : !by_score       ? (double)l[i]
                                        : (softmax ? value64[i] / sum : value64[i]) + (double)b[i];
       if constexpr (kGroups) {
-        kept = groups_kept<L, C>(value64, 0.0f, sub, opt, n_experts, m, close);
+        if (opt.n_groups <= L) kept = groups_kept<L, C>(value64, 0.0f, sub, opt, n_experts, m, close);
         in_kept<C>(kept, sub, n_experts / opt.n_groups, in);
       }
 #pragma unroll

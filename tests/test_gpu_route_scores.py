@@ -217,6 +217,29 @@ def test_balance_bias_evens_out_the_loads(gpu):
     assert load.max() < first.max() // 2
 
 
+def test_logits_off_16_byte_boundaries(gpu):
+    for e, dtype in ((64, torch.bfloat16), (256, torch.float32)):
+        logits, bias = _inputs(gpu, 50, e, dtype, False, True)
+        buf = torch.zeros(50 * e + 1, dtype=dtype, device=gpu)
+        buf[1:] = logits.view(-1)
+        shifted = torch.zeros(e + 1, device=gpu)
+        shifted[1:] = bias
+        a = ops.moe_route_scores(logits, 4, ops.Routing("sigmoid", 8, 4, 2), bias)
+        b = ops.moe_route_scores(buf[1:].view(50, e), 4, ops.Routing("sigmoid", 8, 4, 2), shifted[1:])
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_near_ties_in_every_place(gpu):
+    """Biases that put neighbours of the order, the border of the choice and the
+    border of the groups within 2^-24 of each other: still the 64-bit choice."""
+    gen = torch.Generator().manual_seed(8)
+    for e, routing in ((64, ops.Routing("sigmoid")), (128, ops.Routing("sigmoid", 8, 3, 2)),
+                       (256, ops.Routing("softmax", 8, 4, 1)), (512, ops.Routing("sigmoid", 16, 4, 2))):
+        logits = (torch.randn(300, 1, generator=gen) + 1e-6 * torch.randn(300, e, generator=gen)).to(gpu)
+        bias = (torch.randn(e, generator=gen) * 2.0 ** -26).to(gpu)
+        _check_route(ops.moe_route_scores(logits, 6, routing, bias), logits, 6, routing, bias, torch.float32)
+
+
 def test_no_tokens(gpu):
     r = ops.moe_route_scores(torch.empty(0, 64, device=gpu), 4)
     assert r.topk_idx.shape == (0, 4) and r.chunk_hist.shape == (0, 64)
