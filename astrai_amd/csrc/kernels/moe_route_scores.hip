@@ -253,45 +253,51 @@ __device__ __attribute__((noinline)) void choose_slowly(const T* row, const floa
 
 // Bounds of the error of a difference of two scores: a sigmoid s from exp_near is off
 // by s (1 - s) (|l| 2^-24 + 2^-23) + s (2^-23 + 2^-24) < 2^-22, a softmax by up to 40
-// roundings of its sum and of 1 / sum more. Twice that, and of the biases' additions.
-constexpr float kTolSigmoid = 0x1p-20f, kTolSoftmax = 0x1p-18f, kTolBias = 0x1p-23f;
+// roundings of its sum and of 1 / sum more. Twice that. A value that went through a key
+// is off by 16 units in the last place, 2^-19 of it, and the addition of its bias by
+// 2^-24 (kTolKey).
+constexpr float kTolSigmoid = 0x1p-20f, kTolSoftmax = 0x1p-18f, kTolKey = 0x1.1p-19f;
 
 // Whether two scores or values as near as a and b <= a may be the other way round.
 __device__ __forceinline__ bool near(float a, float b, float tol) {
-  return b > -INFINITY && a - b <= tol + kTolBias * (fabsf(a) + fabsf(b));
+  return b > -INFINITY && a - b <= tol + kTolKey * (fabsf(a) + fabsf(b));
 }
 
-// The groups that stay (as bits; at most 64) from the experts' values (-inf: off). p
-// lanes share a group. `close`: the border lies between two that are near.
+// How the groups lie: `per` experts each; where a group is 2^shift whole lanes, shift,
+// otherwise -1.
+struct GroupShape {
+  int per, shift;
+};
+
+// The two largest of two pairs a1 >= a2, b1 >= b2.
+template <typename F>
+__device__ __forceinline__ void merge_two(F& a1, F& a2, F b1, F b2) {
+  const F low = b1 < a1 ? b1 : a1, high2 = b2 > a2 ? b2 : a2;
+  a2 = low > high2 ? low : high2;
+  a1 = b1 > a1 ? b1 : a1;
+}
+
+// The groups that stay (as bits; at most 64) from the experts' values (-inf: off),
+// however they lie. `close`: the border lies between two that are near.
 template <int L, int C, typename F, typename Lds>
 __device__ __forceinline__ uint64_t groups_kept(const F (&value)[C], float tol, int sub, const astrai_moe_routing& opt,
-                                                int n_experts, Lds& m, bool& close) {
+                                                int per, int n_experts, Lds& m, bool& close) {
   constexpr F kOffKey = (F)-INFINITY;
-  const int per = n_experts / opt.n_groups;
   F* const values = reinterpret_cast<F*>(m.key);
   wave_sync();
 #pragma unroll
   for (int i = 0; i < C; ++i)
     if (sub * C + i < n_experts) values[sub * C + i] = value[i];
   wave_sync();
-  int p = 1;
+  int p = 1;  // lanes of a group
   while (2 * p * opt.n_groups <= L) p *= 2;
   const int g = sub / p;
   F a1 = kOffKey, a2 = kOffKey;
   if (g < opt.n_groups)
-    for (int j = sub & (p - 1); j < per; j += p) {
-      const F v = values[g * per + j];
-      const F low = v < a1 ? v : a1;
-      a2 = low > a2 ? low : a2;
-      a1 = v > a1 ? v : a1;
-    }
-  for (int off = 1; off < p; off *= 2) {
-    const F o1 = __shfl_xor(a1, off, L), o2 = __shfl_xor(a2, off, L);
-    const F low = o1 < a1 ? o1 : a1, high2 = o2 > a2 ? o2 : a2;
-    a2 = low > high2 ? low : high2;
-    a1 = o1 > a1 ? o1 : a1;
-  }
+    for (int j = sub & (p - 1); j < per; j += p) merge_two(a1, a2, values[g * per + j], kOffKey);
+  for (int off = 1; off < p; off *= 2) merge_two(a1, a2, __shfl_xor(a1, off, L), __shfl_xor(a2, off, L));
   F mine = opt.group_top == 2 ? a1 + a2 : a1, last = kOffKey;
+  const float size = mine > kOffKey ? (float)(a1 < 0 ? -a1 : a1) + (opt.group_top == 2 ? (float)(a2 < 0 ? -a2 : a2) : 0.0f) : 0.0f;
   uint64_t kept = 0;
   for (int k = 0; k < opt.topk_groups; ++k) {
     last = lanes_max<L>(mine);
@@ -300,33 +306,43 @@ __device__ __forceinline__ uint64_t groups_kept(const F (&value)[C], float tol, 
     kept |= 1ull << (at & 63);
     if (g == at) mine = kOffKey;
   }
-  if (tol > 0.0f) close = near((float)last, (float)lanes_max<L>(mine), 2.0f * tol);
+  if (tol > 0.0f) {
+    const float next = (float)lanes_max<L>(mine);
+    close = next > -INFINITY && (float)last - next <= 2.0f * tol + 2.0f * kTolKey * lanes_max<L>(size);
+  }
   return kept;
 }
 
-// Whether the lane's i-th expert is in a group that stays.
+// Which of the lane's C experts are in a group that stays, as bits.
 template <int C>
-__device__ __forceinline__ void in_kept(uint64_t kept, int sub, int per, bool (&in)[C]) {
+__device__ __forceinline__ uint32_t in_kept(uint64_t kept, int sub, int per) {
   int g = sub * C / per, left = per - (sub * C - g * per);
+  uint32_t in = 0;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    in[i] = (kept >> (g & 63) & 1) != 0;
+    in |= (uint32_t)(kept >> (g & 63) & 1) << i;
     if (--left == 0) left = per, ++g;
   }
+  return in;
 }
 
-// A float as an integer that orders alike; INT_MIN, below every float's, stands for
-// what is taken or does not exist.
-constexpr int kOff32 = INT32_MIN + 0x7fffff;  // -inf's
-__device__ __forceinline__ int order32(float v) {
-  const int i = __float_as_int(v + 0.0f);  // (-0 as 0)
-  return i ^ (i >> 31 & 0x7fffffff);
+// A key orders like a 32-bit value without its 4 lowest bits, and among equals by
+// the expert's place i in its lane, lower first: these bits hold 15 - i. Exact for logits
+// that were bf16. 0, below every value's, stands for what is taken or does not exist.
+constexpr uint32_t kValueBits = ~15u;
+constexpr uint32_t kOffKey = 0x007ffff0u;  // -inf's
+__device__ __forceinline__ uint32_t key_of(float v, int i) {
+  const int b = __float_as_int(v + 0.0f);  // (-0 as 0)
+  return ((uint32_t)(b ^ (b >> 31 | INT32_MIN)) & kValueBits) | (uint32_t)(15 - i);
 }
-__device__ __forceinline__ float value32(int o) { return __int_as_float(o ^ (o >> 31 & 0x7fffffff)); }
+__device__ __forceinline__ float value_of(uint32_t key) {
+  const uint32_t k = key & kValueBits;
+  return k <= kOffKey ? -INFINITY : __int_as_float((int)(k ^ (~(uint32_t)((int)k >> 31) | 0x80000000u)));
+}
 
-// Sorts a lane's C pairs (key above, ~index below) downwards: odd-even merges.
+// Sorts a lane's C keys downwards: odd-even merges.
 template <int C>
-__device__ __forceinline__ void sort_down(uint64_t (&v)[C]) {
+__device__ __forceinline__ void sort_down(uint32_t (&v)[C]) {
 #pragma unroll
   for (int p = 1; p < C; p *= 2)
 #pragma unroll
@@ -336,35 +352,65 @@ __device__ __forceinline__ void sort_down(uint64_t (&v)[C]) {
 #pragma unroll
         for (int i = 0; i < k; ++i)
           if (i + j + k < C && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-            const uint64_t a = v[i + j], b = v[i + j + k];
-            const bool swap = b > a;
-            v[i + j] = swap ? b : a;
-            v[i + j + k] = swap ? a : b;
+            const uint32_t a = v[i + j], b = v[i + j + k];
+            v[i + j] = max(a, b);
+            v[i + j + k] = min(a, b);
           }
 }
 
-// The top_k experts of the largest keys (INT_MIN: none) into m.pick, their keys as
-// floats into m.score; dead ones (-inf) come last, by their index. Returns the largest
-// key left.
+// Whether the lane's group stays, where groups are whole lanes, from the lanes' sorted
+// keys. The keys are of the scores with their biases (scored), or of logits; then the
+// groups' values are made of these by `score`, unless they go by the logits alone.
+template <int L, int C, typename Score>
+__device__ __forceinline__ bool group_stays(const uint32_t (&v)[C], float tol, bool scored, bool exact, int sub,
+                                            const astrai_moe_routing& opt, int shift, Score score, bool& close) {
+  uint32_t k1 = v[0] & kValueBits, k2 = v[1] & kValueBits;
+  if (shift > 0) merge_two(k1, k2, other<0>(k1), other<0>(k2));
+  if (shift > 1) merge_two(k1, k2, other<1>(k1), other<1>(k2));
+  if (shift > 2) merge_two(k1, k2, other<2>(k1), other<2>(k2));
+  if (shift > 3) merge_two(k1, k2, other<3>(k1), other<3>(k2));
+  if constexpr (L >= 64)
+    if (shift > 4) merge_two(k1, k2, other<4>(k1), other<4>(k2));
+  float a1 = value_of(k1), size = fabsf(a1);  // size: what the keys' roundings are relative to
+  if (opt.group_top == 2) {
+    const float a2 = value_of(k2);
+    const float s1 = scored || a1 == -INFINITY ? a1 : score(a1), s2 = scored || a2 == -INFINITY ? a2 : score(a2);
+    size = scored ? size + fabsf(a2) : s1 * (1.0f + size) + s2 * (1.0f + fabsf(a2));
+    a1 = s1 + s2;
+  }
+  // (the value's order as an integer; 0: taken)
+  uint32_t mine = key_of(a1, 15), last = 0;
+  if (mine <= kOffKey) size = 0.0f;
+  bool stays = false;
+  for (int k = 0; k < opt.topk_groups; ++k) {
+    last = lanes_max<L>(mine);
+    const int at = first_lane<L>(mine == last);
+    if (sub >> shift == at >> shift) mine = 0, stays = true;
+  }
+  const uint32_t next = lanes_max<L>(mine);
+  if (tol > 0.0f)
+    close = next > kOffKey && value_of(last) - value_of(next) <= 2.0f * tol + 4.0f * kTolKey * lanes_max<L>(size);
+  else
+    close = !exact && next > kOffKey && last == next;
+  return stays;
+}
+
+// The top_k experts of the largest keys (0: none) into m.pick, their values into
+// m.score; dead ones (-inf) come last, by their index. Returns the largest value left.
 template <int L, int C, typename Lds>
-__device__ __forceinline__ float pick(const int (&key)[C], int sub, int top_k, Lds& m) {
-  uint64_t v[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) v[i] = (uint64_t)((uint32_t)key[i] ^ 0x80000000u) << 32 | (uint32_t)~(sub * C + i);
-  sort_down(v);
+__device__ __forceinline__ float pick(uint32_t (&v)[C], int sub, int top_k, Lds& m) {
   for (int k = 0; k < top_k; ++k) {
-    const int mine = (int)((uint32_t)(v[0] >> 32) ^ 0x80000000u);
-    const int top = lanes_max<L>(mine);
+    const uint32_t mine = v[0] & kValueBits;
+    const uint32_t top = lanes_max<L>(mine);
     if (sub == first_lane<L>(mine == top)) {
-      m.pick[k] = (int)~(uint32_t)v[0];
-      m.score[k] = value32(top);
+      m.pick[k] = sub * C + 15 - (int)(v[0] & 15);
+      m.score[k] = value_of(top);
 #pragma unroll
       for (int i = 0; i + 1 < C; ++i) v[i] = v[i + 1];
       v[C - 1] = 0;
     }
   }
-  const int left = lanes_max<L>((int)((uint32_t)(v[0] >> 32) ^ 0x80000000u));
-  return left <= kOff32 ? -INFINITY : value32(left);
+  return value_of(lanes_max<L>(v[0]));
 }
 
 // The same from 64-bit keys (-inf: off), for the few tokens that need them.
@@ -435,7 +481,7 @@ template <typename T, typename W, int L, int C, bool kGroups, bool kList>
 __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_kernel(
     const T* __restrict__ logits, const float* __restrict__ bias, const astrai_moe_routing opt, int64_t n_tokens,
     int n_experts, int top_k, int n_shared, int32_t* __restrict__ topk_idx, W* __restrict__ topk_w,
-    int32_t* __restrict__ chunk_hist, const RouteList list, bool vec, bool vec_bias) {
+    int32_t* __restrict__ chunk_hist, const RouteList list, const GroupShape shape, bool vec, bool vec_bias) {
   constexpr int THREADS = score_threads<L, kList>();
   constexpr int TOKENS = THREADS / L < ASTRAI_MOE_CHUNK_TOKENS ? THREADS / L : ASTRAI_MOE_CHUNK_TOKENS;  // in flight
   __shared__ int hist[ASTRAI_MOE_MAX_EXPERTS];  // kList: the experts' first rows
@@ -487,31 +533,66 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
       for (int i = 0; i < C; ++i) sum += l[i] == -INFINITY ? 0.0f : exp_near(l[i] - mx);
       inv = 1.0f / lanes_sum<L>(sum);
     }
+    const auto score = [&](float x) {
+      return softmax ? exp_near(x - mx) * inv : __builtin_amdgcn_rcpf(1.0f + exp_near(-x));
+    };
     const float tol = !by_score ? 0.0f : softmax ? kTolSoftmax : kTolSigmoid;
-    float value[C];  // what groups go by, and with a bias the experts
+    float value[C];  // what the experts go by
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const bool off = l[i] == -INFINITY;
-      const float near_s = softmax ? exp_near(l[i] - mx) * inv : __builtin_amdgcn_rcpf(1.0f + exp_near(-l[i]));
-      value[i] = !by_score || off ? l[i] : near_s + b[i];
-    }
-    int key[C];
-    bool close = false, in[C];
-    uint64_t kept = 0;
+    for (int i = 0; i < C; ++i) value[i] = l[i];
+    if (bias != nullptr)
+#pragma unroll
+      for (int i = 0; i < C; ++i) value[i] = l[i] == -INFINITY ? l[i] : score(l[i]) + b[i];
+    bool close = false;
+    uint32_t in = ~0u;  // the lane's experts in groups that stay
     if constexpr (kGroups) {
-      if (opt.n_groups <= L) kept = groups_kept<L, C>(value, tol, sub, opt, n_experts, m, close);
-      in_kept<C>(kept, sub, n_experts / opt.n_groups, in);
+      if (shape.shift < 0 && opt.n_groups <= L) {
+        float worth[C];  // what the groups go by
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+          worth[i] = by_score && bias == nullptr && l[i] != -INFINITY ? score(l[i]) : value[i];
+        in = in_kept<C>(groups_kept<L, C>(worth, tol, sub, opt, shape.per, n_experts, m, close), sub, shape.per);
+      }
     }
+    uint32_t key[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int k = order32(bias == nullptr ? l[i] : value[i]);
-      key[i] = sub * C + i >= n_experts ? INT32_MIN : kGroups && !in[i] ? kOff32 : k;
+      key[i] = sub * C + i >= n_experts ? 0 : key_of(value[i], i);
+      if constexpr (kGroups) key[i] = key[i] != 0 && (in >> i & 1) == 0 ? kOffKey | (15 - i) : key[i];
+    }
+    sort_down(key);
+    if constexpr (kGroups) {
+      if (shape.shift >= 0 &&
+          !group_stays<L, C>(key, tol, bias != nullptr, sizeof(T) == 2, sub, opt, shape.shift, score, close)) {
+        in = 0;
+#pragma unroll
+        for (int i = 0; i < C; ++i) key[i] = sub * C + i < n_experts ? kOffKey | (15 - i) : 0;
+      }
     }
     const float left_out = pick<L, C>(key, sub, top_k, m);
     wave_sync();
-    if (bias != nullptr)
-      for (int k = sub; k < top_k; k += L)
-        close |= near(m.score[k], k + 1 < top_k ? m.score[k + 1] : left_out, tol);
+    if (bias != nullptr || sizeof(T) == 4) {
+      // (logits alone: only what their keys leave out)
+      const auto apart = [&](float a, float b) { return bias != nullptr ? near(a, b, tol) : b > -INFINITY && a == b; };
+      const T* const row = logits + (on ? t : t_begin) * n_experts;
+      for (int k = sub; k + 1 < top_k; k += L)
+        if (apart(m.score[k], m.score[k + 1])) {  // (alike in logit and bias: the lower expert came first)
+          const int e0 = min(m.pick[k], n_experts - 1), e1 = min(m.pick[k + 1], n_experts - 1);  // (odd rows')
+          close |= Elem<T>::to_f32(row[e0]) != Elem<T>::to_f32(row[e1]) || (bias != nullptr && bias[e0] != bias[e1]);
+        }
+      const float a = m.score[top_k - 1];
+      if (apart(a, left_out)) {
+        const int e = min(m.pick[top_k - 1], n_experts - 1);
+        const float la = Elem<T>::to_f32(row[e]), ba = bias != nullptr ? bias[e] : 0.0f;
+        const uint32_t ka = key_of(a, 15);
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const uint32_t ki = key_of(value[i], 15);
+          const bool left = (in >> i & 1) != 0 && (ki < ka || (ki == ka && sub * C + i > e));
+          close |= left && apart(a, value_of(ki)) && (l[i] != la || b[i] != ba);
+        }
+      }
+    }
     if (__ballot(close && on) != 0) {  // (the wave's other tokens get the choice that they have)
       double value64[C], key64[C], sum = 0.0;
 #pragma unroll
@@ -526,13 +607,14 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
         value64[i] = l[i] == -INFINITY ? -INFINITY
                      : !by_score       ? (double)l[i]
                                        : (softmax ? value64[i] / sum : value64[i]) + (double)b[i];
+      in = ~0u;
       if constexpr (kGroups) {
-        if (opt.n_groups <= L) kept = groups_kept<L, C>(value64, 0.0f, sub, opt, n_experts, m, close);
-        in_kept<C>(kept, sub, n_experts / opt.n_groups, in);
+        if (opt.n_groups <= L)
+          in = in_kept<C>(groups_kept<L, C>(value64, 0.0f, sub, opt, shape.per, n_experts, m, close), sub, shape.per);
       }
 #pragma unroll
       for (int i = 0; i < C; ++i)
-        key64[i] = kGroups && !in[i] ? -INFINITY : bias == nullptr ? (double)l[i] : value64[i];
+        key64[i] = (in >> i & 1) == 0 ? -INFINITY : bias == nullptr ? (double)l[i] : value64[i];
       pick64<L, C>(key64, sub, n_experts, top_k, m);
       wave_sync();
     }
@@ -696,9 +778,11 @@ void launch_scores_cfg(const void* logits, const float* bias, const astrai_moe_r
                     ? (list != nullptr ? &route_scores_kernel<T, W, L, C, true, true> : &route_scores_kernel<T, W, L, C, true, false>)
                     : (list != nullptr ? &route_scores_kernel<T, W, L, C, false, true> : &route_scores_kernel<T, W, L, C, false, false>);
   const int threads = list != nullptr ? score_threads<L, true>() : score_threads<L, false>();
+  GroupShape shape{n_experts / opt.n_groups, -1};
+  if (shape.per % C == 0 && (shape.per / C & (shape.per / C - 1)) == 0) shape.shift = __builtin_ctz(shape.per / C);
   hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, static_cast<const T*>(logits), bias, opt, n_tokens, n_experts,
                      top_k, n_shared, topk_idx, static_cast<W*>(topk_w), chunk_hist,
-                     list != nullptr ? *list : RouteList{},
+                     list != nullptr ? *list : RouteList{}, shape,
                      n_experts * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0,
                      n_experts % 4 == 0 && reinterpret_cast<uintptr_t>(bias) % 16 == 0);
 }

@@ -240,6 +240,51 @@ def test_near_ties_in_every_place(gpu):
         _check_route(ops.moe_route_scores(logits, 6, routing, bias), logits, 6, routing, bias, torch.float32)
 
 
+@pytest.mark.parametrize("e,groups,kept", [(32, 4, 2), (64, 8, 3), (64, 4, 2), (128, 2, 1), (256, 8, 4), (256, 2, 1),
+                                           (256, 16, 5), (192, 6, 2), (512, 2, 1), (512, 16, 4), (1024, 2, 1),
+                                           (1024, 32, 8), (160, 8, 3), (96, 32, 9)])
+@pytest.mark.parametrize("top", [1, 2])
+def test_groups_of_every_width(gpu, e, groups, kept, top):
+    """Groups of part of a lane's experts up to half of all lanes', coarse logits with
+    many exact ties, with and without a bias, some experts off."""
+    gen = torch.Generator().manual_seed(e + groups)
+    for score in ("sigmoid", "softmax"):
+        routing = ops.Routing(score, groups, kept, top)
+        for dtype in (torch.bfloat16, torch.float32):
+            for bias in (None, torch.zeros(e, device=gpu), torch.randn(e, generator=gen).to(gpu)):
+                logits = torch.randn(70, e, generator=gen).to(torch.bfloat16).to(dtype)
+                logits[torch.rand(70, e, generator=gen) < 0.1] = -math.inf
+                logits = logits.to(gpu)
+                _check_route(ops.moe_route_scores(logits, 3, routing, bias), logits, 3, routing, bias, dtype)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_logits_that_differ_in_their_last_bits(gpu, score):
+    """Neighbours a unit in the last place apart, at every size: the larger first,
+    also of group maxima."""
+    gen = torch.Generator().manual_seed(4)
+    for e, routing in ((64, ops.Routing(score)), (128, ops.Routing(score, 8, 3, 1)), (60, ops.Routing(score, 6, 2, 1)),
+                       (256, ops.Routing(score, 8, 4, 2))):
+        base = torch.randn(200, 1, generator=gen)
+        steps = torch.randint(-20, 20, (200, e), generator=gen, dtype=torch.int32)
+        logits = (base.view(torch.int32) + steps).view(torch.float32).to(gpu)
+        _check_route(ops.moe_route_scores(logits, 6, routing), logits, 6, routing, None, torch.float32)
+
+
+def test_large_biases_that_cancel_in_a_group(gpu):
+    """Group values whose parts are far larger than their sums: rounded in 32 bits they
+    lose what tells the groups apart."""
+    gen = torch.Generator().manual_seed(6)
+    for e, groups in ((64, 8), (160, 8)):
+        per = e // groups
+        bias = torch.full((e,), -4096.0)
+        bias[::per], bias[1::per] = 4096.0, -4095.0
+        logits = torch.randn(200, e, generator=gen).to(gpu)
+        routing = ops.Routing("sigmoid", groups, 3, 2)
+        bias = bias.to(gpu)
+        _check_route(ops.moe_route_scores(logits, 4, routing, bias), logits, 4, routing, bias, torch.float32)
+
+
 def test_no_tokens(gpu):
     r = ops.moe_route_scores(torch.empty(0, 64, device=gpu), 4)
     assert r.topk_idx.shape == (0, 4) and r.chunk_hist.shape == (0, 64)
