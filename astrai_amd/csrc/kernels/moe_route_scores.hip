@@ -73,10 +73,12 @@ __device__ __forceinline__ float other(float v) {
   return __builtin_bit_cast(float, other<STEP>(__builtin_bit_cast(unsigned, v)));
 }
 template <int STEP>
+__device__ __forceinline__ uint64_t other(uint64_t v) {
+  return (uint64_t)other<STEP>((unsigned)(v >> 32)) << 32 | other<STEP>((unsigned)v);
+}
+template <int STEP>
 __device__ __forceinline__ double other(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint64_t o = (uint64_t)other<STEP>((unsigned)(u >> 32)) << 32 | other<STEP>((unsigned)u);
-  return __builtin_bit_cast(double, o);
+  return __builtin_bit_cast(double, other<STEP>(__builtin_bit_cast(uint64_t, v)));
 }
 
 // op over the L lanes of a token, in every one of them. Needs the whole wave.
@@ -253,12 +255,12 @@ __device__ __attribute__((noinline)) void choose_slowly(const T* row, const floa
 
 // Bounds of the error of a difference of two scores: a sigmoid s from exp_near is off
 // by s (1 - s) (|l| 2^-24 + 2^-23) + s (2^-23 + 2^-24) < 2^-22, a softmax by up to 40
-// roundings of its sum and of 1 / sum more. Twice that. A value that went through a key
-// is off by 16 units in the last place, 2^-19 of it, and the addition of its bias by
-// 2^-24 (kTolKey).
-constexpr float kTolSigmoid = 0x1p-20f, kTolSoftmax = 0x1p-18f, kTolKey = 0x1.1p-19f;
+// roundings of its sum and of 1 / sum more, relative to the row's largest score (the
+// largest 1 / sum). The addition of a bias: half a step (kTolAdd: doubled). A value that
+// went through a key is off by 16 units in the last place, 2^-19 of it, and that (kTolKey).
+constexpr float kTolSigmoid = 0x1p-21f, kTolSoftmax = 0x1p-18f, kTolAdd = 0x1p-23f, kTolKey = 0x1.1p-19f;
 
-// Whether two scores or values as near as a and b <= a may be the other way round.
+// Whether two values that went through keys, a and b <= a, may be the other way round.
 __device__ __forceinline__ bool near(float a, float b, float tol) {
   return b > -INFINITY && a - b <= tol + kTolKey * (fabsf(a) + fabsf(b));
 }
@@ -277,40 +279,70 @@ __device__ __forceinline__ void merge_two(F& a1, F& a2, F b1, F b2) {
   a1 = b1 > a1 ? b1 : a1;
 }
 
-// The groups that stay (as bits; at most 64) from the experts' values (-inf: off),
-// however they lie. `close`: the border lies between two that are near.
-template <int L, int C, typename F, typename Lds>
-__device__ __forceinline__ uint64_t groups_kept(const F (&value)[C], float tol, int sub, const astrai_moe_routing& opt,
-                                                int per, int n_experts, Lds& m, bool& close) {
-  constexpr F kOffKey = (F)-INFINITY;
-  F* const values = reinterpret_cast<F*>(m.key);
-  wave_sync();
-#pragma unroll
-  for (int i = 0; i < C; ++i)
-    if (sub * C + i < n_experts) values[sub * C + i] = value[i];
-  wave_sync();
-  int p = 1;  // lanes of a group
-  while (2 * p * opt.n_groups <= L) p *= 2;
-  const int g = sub / p;
-  F a1 = kOffKey, a2 = kOffKey;
-  if (g < opt.n_groups)
-    for (int j = sub & (p - 1); j < per; j += p) merge_two(a1, a2, values[g * per + j], kOffKey);
-  for (int off = 1; off < p; off *= 2) merge_two(a1, a2, __shfl_xor(a1, off, L), __shfl_xor(a2, off, L));
-  F mine = opt.group_top == 2 ? a1 + a2 : a1, last = kOffKey;
-  const float size = mine > kOffKey ? (float)(a1 < 0 ? -a1 : a1) + (opt.group_top == 2 ? (float)(a2 < 0 ? -a2 : a2) : 0.0f) : 0.0f;
+// The best topk_groups of the groups' values (p lanes a group; -inf: no live expert) as
+// bits; `last` is the least of them and `next` the best of the others.
+template <int L, typename F>
+__device__ __forceinline__ uint64_t best_groups(F mine, int g, int p, int topk_groups, F& last, F& next) {
+  constexpr F kDead = (F)-INFINITY;
   uint64_t kept = 0;
-  for (int k = 0; k < opt.topk_groups; ++k) {
+  for (int k = 0; k < topk_groups; ++k) {
     last = lanes_max<L>(mine);
     // (groups without live experts: the lowest not kept yet)
-    const int at = last > kOffKey ? first_lane<L>(mine == last) / p : __builtin_ctzll(~kept);
+    const int at = last > kDead ? first_lane<L>(mine == last) / p : __builtin_ctzll(~kept);
     kept |= 1ull << (at & 63);
-    if (g == at) mine = kOffKey;
+    if (g == at) mine = kDead;
   }
-  if (tol > 0.0f) {
-    const float next = (float)lanes_max<L>(mine);
-    close = next > -INFINITY && (float)last - next <= 2.0f * tol + 2.0f * kTolKey * lanes_max<L>(size);
-  }
+  next = lanes_max<L>(mine);
   return kept;
+}
+
+// The groups that stay (as bits; at most 64) from the experts' values (-inf: off),
+// however they lie. Where the border of a token of the wave lies between two that are
+// near, again from exact(expert, sum64()), of each group's experts that may be its best.
+template <int L, int C, typename Lds, typename Sum, typename Exact>
+__device__ __forceinline__ uint64_t groups_kept(const float (&value)[C], float tol, int sub,
+                                                const astrai_moe_routing& opt, int per, int n_experts, bool on, Lds& m,
+                                                Sum sum64, Exact exact) {
+  float* const values = reinterpret_cast<float*>(m.key);
+  const auto store = [&] {
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (sub * C + i < n_experts) values[sub * C + i] = value[i];
+    wave_sync();
+  };
+  store();
+  int p = 1;  // lanes of a group
+  while (2 * p * opt.n_groups <= L) p *= 2;
+  const int g = sub / p, begin = g < opt.n_groups ? sub & (p - 1) : per;
+  const bool two = opt.group_top == 2;
+  float a1 = -INFINITY, a2 = -INFINITY;
+  for (int j = begin; j < per; j += p) merge_two(a1, a2, values[g * per + j], -INFINITY);
+  for (int off = 1; off < p; off *= 2) merge_two(a1, a2, __shfl_xor(a1, off, L), __shfl_xor(a2, off, L));
+  const float mine = two ? a1 + a2 : a1;
+  float last, next;
+  const uint64_t kept = best_groups<L>(mine, g, p, opt.topk_groups, last, next);
+  if (tol == 0.0f) return kept;
+  const float size = lanes_max<L>(mine > -INFINITY ? fabsf(a1) + (two ? fabsf(a2) : 0.0f) : 0.0f);
+  if (__ballot(on && next > -INFINITY && last - next <= 2.0f * tol + 4.0f * kTolAdd * size) == 0) return kept;
+  const double sum = sum64();
+  store();
+  const float least = two ? a2 : a1;
+  double d1 = -INFINITY, d2 = -INFINITY;
+  for (int j = begin;;) {
+    for (; j < per; j += p) {
+      const float v = values[g * per + j];
+      if (v > -INFINITY && least - v <= tol + kTolAdd * (fabsf(v) + fabsf(least))) break;
+    }
+    if (__ballot(j < per) == 0) break;
+    if (j < per) {
+      merge_two(d1, d2, exact(g * per + j, sum), (double)-INFINITY);
+      j += p;
+    }
+  }
+  for (int off = 1; off < p; off *= 2) merge_two(d1, d2, __shfl_xor(d1, off, L), __shfl_xor(d2, off, L));
+  double last64, next64;
+  return best_groups<L>(two ? d1 + d2 : d1, g, p, opt.topk_groups, last64, next64);
 }
 
 // Which of the lane's C experts are in a group that stays, as bits.
@@ -326,18 +358,23 @@ __device__ __forceinline__ uint32_t in_kept(uint64_t kept, int sub, int per) {
   return in;
 }
 
-// A key orders like a 32-bit value without its 4 lowest bits, and among equals by
-// the expert's place i in its lane, lower first: these bits hold 15 - i. Exact for logits
-// that were bf16. 0, below every value's, stands for what is taken or does not exist.
+// A float as an unsigned integer that orders alike; 0, below every float's, stands for
+// what is taken or does not exist.
+__device__ __forceinline__ uint32_t bits_of(float v) {
+  const int b = __float_as_int(v + 0.0f);  // (-0 as 0)
+  return (uint32_t)(b ^ (b >> 31 | INT32_MIN));
+}
+__device__ __forceinline__ float float_of(uint32_t o) {
+  return __int_as_float((int)(o ^ (~(uint32_t)((int)o >> 31) | 0x80000000u)));
+}
+// A key orders like a value without its 4 lowest bits, and among equals by the
+// expert's place i in its lane, lower first: these bits hold 15 - i. Exact for logits that
+// were bf16.
 constexpr uint32_t kValueBits = ~15u;
 constexpr uint32_t kOffKey = 0x007ffff0u;  // -inf's
-__device__ __forceinline__ uint32_t key_of(float v, int i) {
-  const int b = __float_as_int(v + 0.0f);  // (-0 as 0)
-  return ((uint32_t)(b ^ (b >> 31 | INT32_MIN)) & kValueBits) | (uint32_t)(15 - i);
-}
+__device__ __forceinline__ uint32_t key_of(float v, int i) { return (bits_of(v) & kValueBits) | (uint32_t)(15 - i); }
 __device__ __forceinline__ float value_of(uint32_t key) {
-  const uint32_t k = key & kValueBits;
-  return k <= kOffKey ? -INFINITY : __int_as_float((int)(k ^ (~(uint32_t)((int)k >> 31) | 0x80000000u)));
+  return (key & kValueBits) <= kOffKey ? -INFINITY : float_of(key & kValueBits);
 }
 
 // Sorts a lane's C keys downwards: odd-even merges.
@@ -358,40 +395,42 @@ __device__ __forceinline__ void sort_down(uint32_t (&v)[C]) {
           }
 }
 
-// Whether the lane's group stays, where groups are whole lanes, from the lanes' sorted
-// keys. The keys are of the scores with their biases (scored), or of logits; then the
-// groups' values are made of these by `score`, unless they go by the logits alone.
+// Whether the lane's group stays, where groups are 2^shift whole lanes, from what the
+// experts go by (-inf: off): logits, whose `score` groups of two go by, or scores with
+// their biases (scored). `close`: the border lies between two that are near.
 template <int L, int C, typename Score>
-__device__ __forceinline__ bool group_stays(const uint32_t (&v)[C], float tol, bool scored, bool exact, int sub,
+__device__ __forceinline__ bool group_stays(const float (&value)[C], float tol, bool scored, int sub,
                                             const astrai_moe_routing& opt, int shift, Score score, bool& close) {
-  uint32_t k1 = v[0] & kValueBits, k2 = v[1] & kValueBits;
-  if (shift > 0) merge_two(k1, k2, other<0>(k1), other<0>(k2));
-  if (shift > 1) merge_two(k1, k2, other<1>(k1), other<1>(k2));
-  if (shift > 2) merge_two(k1, k2, other<2>(k1), other<2>(k2));
-  if (shift > 3) merge_two(k1, k2, other<3>(k1), other<3>(k2));
+  float a1 = value[0], a2 = -INFINITY;
+#pragma unroll
+  for (int i = 1; i < C; ++i) {
+    a2 = __builtin_amdgcn_fmed3f(a1, a2, value[i]);
+    a1 = fmaxf(a1, value[i]);
+  }
+  if (shift > 0) merge_two(a1, a2, other<0>(a1), other<0>(a2));
+  if (shift > 1) merge_two(a1, a2, other<1>(a1), other<1>(a2));
+  if (shift > 2) merge_two(a1, a2, other<2>(a1), other<2>(a2));
+  if (shift > 3) merge_two(a1, a2, other<3>(a1), other<3>(a2));
   if constexpr (L >= 64)
-    if (shift > 4) merge_two(k1, k2, other<4>(k1), other<4>(k2));
-  float a1 = value_of(k1), size = fabsf(a1);  // size: what the keys' roundings are relative to
+    if (shift > 4) merge_two(a1, a2, other<4>(a1), other<4>(a2));
+  float size = fabsf(a1);  // (what the sums' roundings are relative to)
   if (opt.group_top == 2) {
-    const float a2 = value_of(k2);
     const float s1 = scored || a1 == -INFINITY ? a1 : score(a1), s2 = scored || a2 == -INFINITY ? a2 : score(a2);
-    size = scored ? size + fabsf(a2) : s1 * (1.0f + size) + s2 * (1.0f + fabsf(a2));
+    size = fabsf(s1) + fabsf(s2);
     a1 = s1 + s2;
   }
-  // (the value's order as an integer; 0: taken)
-  uint32_t mine = key_of(a1, 15), last = 0;
-  if (mine <= kOffKey) size = 0.0f;
+  uint32_t mine = bits_of(a1), last = 0;
+  if (a1 == -INFINITY) size = 0.0f;
   bool stays = false;
   for (int k = 0; k < opt.topk_groups; ++k) {
     last = lanes_max<L>(mine);
     const int at = first_lane<L>(mine == last);
     if (sub >> shift == at >> shift) mine = 0, stays = true;
   }
-  const uint32_t next = lanes_max<L>(mine);
-  if (tol > 0.0f)
-    close = next > kOffKey && value_of(last) - value_of(next) <= 2.0f * tol + 4.0f * kTolKey * lanes_max<L>(size);
-  else
-    close = !exact && next > kOffKey && last == next;
+  if (tol > 0.0f) {
+    const float next = float_of(max(lanes_max<L>(mine), bits_of(-INFINITY)));
+    close = next > -INFINITY && float_of(last) - next <= 2.0f * tol + 4.0f * kTolAdd * lanes_max<L>(size);
+  }
   return stays;
 }
 
@@ -413,29 +452,30 @@ __device__ __forceinline__ float pick(uint32_t (&v)[C], int sub, int top_k, Lds&
   return value_of(lanes_max<L>(v[0]));
 }
 
-// The same from 64-bit keys (-inf: off), for the few tokens that need them.
-template <int L, int C, typename Lds>
-__device__ __forceinline__ void pick64(double (&key)[C], int sub, int n_experts, int top_k, Lds& m) {
-  uint32_t open = 0;  // the lane's experts not chosen yet
-#pragma unroll
-  for (int i = 0; i < C; ++i) open |= sub * C + i < n_experts ? 1u << i : 0u;
+// The same from the exact values of the experts that may be chosen (`open`, bits of the
+// lane's), for the few tokens that need them.
+template <int L, int C, typename Lds, typename Exact>
+__device__ __forceinline__ void pick_exact(uint32_t open, int sub, int top_k, Lds& m, Exact exact) {
+#pragma unroll 1
+  for (uint32_t left = open; __ballot(left != 0) != 0; left &= left - 1)
+    if (left != 0) {
+      const int e = sub * C + __builtin_ctz(left);
+      m.key[e] = order_of(exact(e));
+    }
+#pragma unroll 1
   for (int k = 0; k < top_k; ++k) {
-    double best = key[0];
-#pragma unroll
-    for (int i = 1; i < C; ++i) best = key[i] > best ? key[i] : best;
-    const double top = lanes_max<L>(best);
-    const bool live = top > -INFINITY;
-    if (sub == first_lane<L>(live ? best == top : open != 0)) {
-      int at = live ? 0 : __builtin_ctz(open);
-      if (live)
-#pragma unroll
-        for (int i = C - 1; i >= 0; --i) at = key[i] == top ? i : at;
+    uint64_t best = kNone;
+    int at = 0;
+#pragma unroll 1
+    for (uint32_t left = open; left != 0; left &= left - 1) {
+      const int i = __builtin_ctz(left);
+      if (m.key[sub * C + i] > best) best = m.key[sub * C + i], at = i;
+    }
+    const uint64_t top = lanes_max<L>(best);
+    if (sub == first_lane<L>(best == top) && top != kNone) {
       m.pick[k] = sub * C + at;
-      m.score[k] = (float)top;
+      m.score[k] = (float)value_of(top);
       open &= ~(1u << at);
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (i == at) key[i] = -INFINITY;
     }
   }
 }
@@ -536,87 +576,107 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
     const auto score = [&](float x) {
       return softmax ? exp_near(x - mx) * inv : __builtin_amdgcn_rcpf(1.0f + exp_near(-x));
     };
-    const float tol = !by_score ? 0.0f : softmax ? kTolSoftmax : kTolSigmoid;
+    const float tol = !by_score ? 0.0f : softmax ? kTolSoftmax * inv : kTolSigmoid;
     float value[C];  // what the experts go by
 #pragma unroll
     for (int i = 0; i < C; ++i) value[i] = l[i];
     if (bias != nullptr)
 #pragma unroll
       for (int i = 0; i < C; ++i) value[i] = l[i] == -INFINITY ? l[i] : score(l[i]) + b[i];
-    bool close = false;
+    const T* const row = logits + (on ? t : t_begin) * n_experts;
+    // what decides near ties: a softmax's sum and the value of an expert in 64 bits
+    const auto sum64 = [&] {
+      double sum = 0.0;
+      if (softmax) {
+        float* const values = reinterpret_cast<float*>(m.key);
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < C; ++i) values[sub * C + i] = l[i];
+        wave_sync();
+#pragma unroll 1
+        for (int i = 0; i < C; ++i) {
+          const float x = values[sub * C + i];
+          if (x != -INFINITY) sum += exp((double)x - (double)mx);
+        }
+        sum = lanes_sum<L>(sum);
+        wave_sync();
+      }
+      return sum;
+    };
+    const auto exact = [&](int e, double sum) {
+      const double x = Elem<T>::to_f32(row[e]);
+      return x == -INFINITY ? x : score_of(x, softmax, mx, sum) + (bias != nullptr ? (double)bias[e] : 0.0);
+    };
+    uint32_t key[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) key[i] = sub * C + i >= n_experts ? 0 : key_of(value[i], i);
     uint32_t in = ~0u;  // the lane's experts in groups that stay
     if constexpr (kGroups) {
-      if (shape.shift < 0 && opt.n_groups <= L) {
+      bool again = opt.n_groups <= L;
+      if (shape.shift >= 0) {
+        bool close = false;
+        in = group_stays<L, C>(value, tol, bias != nullptr, sub, opt, shape.shift, score, close) ? ~0u : 0u;
+        again = __ballot(close && on) != 0;
+      }
+      if (again) {
         float worth[C];  // what the groups go by
 #pragma unroll
         for (int i = 0; i < C; ++i)
           worth[i] = by_score && bias == nullptr && l[i] != -INFINITY ? score(l[i]) : value[i];
-        in = in_kept<C>(groups_kept<L, C>(worth, tol, sub, opt, shape.per, n_experts, m, close), sub, shape.per);
+        in = in_kept<C>(groups_kept<L, C>(worth, tol, sub, opt, shape.per, n_experts, on, m, sum64, exact), sub,
+                        shape.per);
       }
-    }
-    uint32_t key[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      key[i] = sub * C + i >= n_experts ? 0 : key_of(value[i], i);
-      if constexpr (kGroups) key[i] = key[i] != 0 && (in >> i & 1) == 0 ? kOffKey | (15 - i) : key[i];
+      for (int i = 0; i < C; ++i) key[i] = key[i] != 0 && (in >> i & 1) == 0 ? kOffKey | (15 - i) : key[i];
     }
     sort_down(key);
-    if constexpr (kGroups) {
-      if (shape.shift >= 0 &&
-          !group_stays<L, C>(key, tol, bias != nullptr, sizeof(T) == 2, sub, opt, shape.shift, score, close)) {
-        in = 0;
-#pragma unroll
-        for (int i = 0; i < C; ++i) key[i] = sub * C + i < n_experts ? kOffKey | (15 - i) : 0;
-      }
-    }
     const float left_out = pick<L, C>(key, sub, top_k, m);
     wave_sync();
     if (bias != nullptr || sizeof(T) == 4) {
       // (logits alone: only what their keys leave out)
       const auto apart = [&](float a, float b) { return bias != nullptr ? near(a, b, tol) : b > -INFINITY && a == b; };
-      const T* const row = logits + (on ? t : t_begin) * n_experts;
-      for (int k = sub; k + 1 < top_k; k += L)
-        if (apart(m.score[k], m.score[k + 1])) {  // (alike in logit and bias: the lower expert came first)
-          const int e0 = min(m.pick[k], n_experts - 1), e1 = min(m.pick[k + 1], n_experts - 1);  // (odd rows')
-          close |= Elem<T>::to_f32(row[e0]) != Elem<T>::to_f32(row[e1]) || (bias != nullptr && bias[e0] != bias[e1]);
-        }
       const float a = m.score[top_k - 1];
-      if (apart(a, left_out)) {
-        const int e = min(m.pick[top_k - 1], n_experts - 1);
-        const float la = Elem<T>::to_f32(row[e]), ba = bias != nullptr ? bias[e] : 0.0f;
-        const uint32_t ka = key_of(a, 15);
+      bool seen = apart(a, left_out), close = false;
+      for (int k = sub; k + 1 < top_k; k += L) seen |= apart(m.score[k], m.score[k + 1]);
+      if (__ballot(seen && on) != 0) {
+        // on the values themselves (their keys may have them in the wrong order); two alike
+        // in logit and bias are in order
+        const auto swapped = [&](float v0, float v1) {
+          return bias == nullptr || v0 - v1 <= tol + kTolAdd * (fabsf(v0) + fabsf(v1));
+        };
+        const auto look = [&](int k, float& l0, float& b0) {
+          const int e = min(m.pick[k], n_experts - 1);  // (odd rows hold anything)
+          l0 = Elem<T>::to_f32(row[e]), b0 = bias != nullptr ? bias[e] : 0.0f;
+          return e;
+        };
+        float l0, b0, l1, b1;
+        for (int k = sub; k + 1 < top_k; k += L)
+          if (apart(m.score[k], m.score[k + 1])) {
+            look(k, l0, b0), look(k + 1, l1, b1);
+            close |= (l0 != l1 || b0 != b1) && swapped(score(l0) + b0, score(l1) + b1);
+          }
+        const int e0 = look(top_k - 1, l0, b0);
+        const float v0 = score(l0) + b0;
+        const uint32_t k0 = key_of(a, 15);
+        uint32_t open = 0;  // the lane's experts that may be among the chosen
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-          const uint32_t ki = key_of(value[i], 15);
-          const bool left = (in >> i & 1) != 0 && (ki < ka || (ki == ka && sub * C + i > e));
-          close |= left && apart(a, value_of(ki)) && (l[i] != la || b[i] != ba);
+          const bool stays = (in >> i & 1) != 0;
+          const uint32_t ki = stays ? key_of(value[i], 15) : kOffKey;
+          const bool beside = apart(a, value_of(ki)), left = ki < k0 || (ki == k0 && sub * C + i > e0);
+          if (sub * C + i < n_experts && (ki >= k0 || beside)) open |= 1u << i;
+          close |= beside && left && (l[i] != l0 || b[i] != b0) && swapped(v0, value[i]);
+        }
+        if (__ballot(close && on) != 0) {  // (the wave's other tokens get the choice that they have)
+          const double sum = bias != nullptr ? sum64() : 0.0;
+          pick_exact<L, C>(open, sub, top_k, m, [&](int e) {
+            return (in >> (e - sub * C) & 1) == 0 ? -INFINITY
+                   : bias != nullptr              ? exact(e, sum)
+                                                  : (double)Elem<T>::to_f32(row[e]);
+          });
+          wave_sync();
         }
       }
-    }
-    if (__ballot(close && on) != 0) {  // (the wave's other tokens get the choice that they have)
-      double value64[C], key64[C], sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const double x = l[i];
-        value64[i] = l[i] == -INFINITY ? 0.0 : softmax ? exp(x - (double)mx) : 1.0 / (1.0 + exp(-x));
-        sum += value64[i];
-      }
-      if (softmax) sum = lanes_sum<L>(sum);
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        value64[i] = l[i] == -INFINITY ? -INFINITY
-                     : !by_score       ? (double)l[i]
-                                       : (softmax ? value64[i] / sum : value64[i]) + (double)b[i];
-      in = ~0u;
-      if constexpr (kGroups) {
-        if (opt.n_groups <= L)
-          in = in_kept<C>(groups_kept<L, C>(value64, 0.0f, sub, opt, shape.per, n_experts, m, close), sub, shape.per);
-      }
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        key64[i] = (in >> i & 1) == 0 ? -INFINITY : bias == nullptr ? (double)l[i] : value64[i];
-      pick64<L, C>(key64, sub, n_experts, top_k, m);
-      wave_sync();
     }
     const uint64_t odd_lanes = __ballot(odd && on);
     if (odd_lanes != 0) {
