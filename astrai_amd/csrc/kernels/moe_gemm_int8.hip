@@ -244,7 +244,11 @@ __device__ __forceinline__ void store_sums(const i32x4_t (&acc)[WM / 16][WN / 16
 }
 
 // ===========================================================================
-// 32-, 64- and 128-row tiles: every wave issues DMA, several stages in flight.
+// 32-, 64- and 128-row tiles: every wave issues DMA, several stages in flight. Bound by
+// reading the weights where an expert has few rows (64 tokens, 128 experts, top-8, D
+// 4096, F 1536: 2.4 GB of codes, the layer 405 us, 5.9 TB/s, as a plain read), by the
+// rounds of tiles otherwise (333 tokens, 64 experts, top-6 and a shared one, D 2048, F
+// 1408: 77 and 47 us of 157; 32- and 128-row tiles there, or a stage more, took as long).
 // ===========================================================================
 template <int BM_, int BN_, int STAGES_, int WGM_, int WGN_, int GM_>
 struct TileCfg {
@@ -446,7 +450,14 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(const Args p) 
 // Streaming kernel: 256 x 256 tiles, 8 matrix-core waves + 4 DMA waves, as
 // gemm_stream_kernel of moe_gemm_mfma.hip, whose comments give the reasons of its
 // schedule: two activation and three weight stages, one barrier a K step, the
-// matrix-core waves' fragments in rings, the priority drops.
+// matrix-core waves' fragments in rings, the priority drops. 16384 tokens, 8 experts,
+// top-2, D 4096, F 14336: gate/up 2.90 to 3.04 ms (2.5 to 2.65 Pop/s), down 1.32 to 1.40
+// (2.75 to 2.9); one expert, 8192 rows, 4096 to 14336 364 to 427 us (2.25 to 2.64). A
+// K step of a tile takes 1.54 us, of which the matrix instructions alone, with their
+// operands in registers on every compute unit at once, take 1.07 (4.0 Pop/s; those of
+// 32 x 32 x 32 3.5); a tile's epilogue and first fragments take 5 us, the tenth by
+// which the shorter K of the gate/up product falls behind (matrix cores busy 73%, down
+// 85%).
 // ===========================================================================
 template <bool kGateUp>
 struct StreamCfg {
@@ -958,7 +969,10 @@ __global__ __launch_bounds__(Cfg::WAVES * 64, 1) void gemm_i8_few_kernel(const A
 // A few tokens: the product quantises its rows itself. Every workgroup reads the (at
 // most 16) rows of its row tile, whose codes stay in LDS, behind its first weight
 // loads: for one token the launch and the trip through memory that a quantiser of its
-// own takes (4 to 5 us) are most of a small product's time. Otherwise as above.
+// own takes (4 to 5 us) are most of a small product's time. Otherwise as above. The rows
+// are held in two units of 512 values a wave (UNITS), where it breaks even (us a product,
+// so / with a quantiser: 4096 to 14336, 1 row 17 / 20; 2048 x 2 rows 8.6 / 8.2; 1024 x 4
+// 6.5 / 7.0, x 8 8.7 / 7.0; 512 x 4 5.2 / 5.9, x 8 6.4 / 5.9).
 // ===========================================================================
 struct QuantCfg {
   static constexpr int BM = 16, BN = 32, WAVES = 4, STAGES = 8, UNITS = 2;

@@ -133,7 +133,6 @@ struct Unit {
   }
 };
 
-
 // On the matrix cores (moe_gemm_int8.hip); gate/up products are gathered (row_src),
 // the others not. a under 4 GiB where gathered. ragged: rows of a partial K step, or
 // outputs whose rows are no whole number of 16 bytes.

@@ -35,8 +35,9 @@ struct ScaleOut {
 
 // One row per WAVES waves, held in registers between its maximum and its codes: a
 // thread has NV units of 8 columns, WAVES * 512 columns apart. kVec: rows start on
-// 16-byte boundaries. clear: a counter of the product that follows, set to 0. One read of x and one write of the codes, bound by these: 117 M
-// values of 8192 rows 100 us, 32768 rows of 14336 XX us (XX TB/s).
+// 16-byte boundaries. clear: a counter of the product that follows, set to 0. One read
+// of x and one write of the codes, bound by these: bf16, 8192 rows of 4096 25 to 28 us
+// (3.8 TB/s), 32768 of 14336 255 to 282 us (5.0 to 5.5 TB/s; a large copy reaches 5.2).
 template <typename T, int WAVES, int NV, bool kVec>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
                                                             int64_t kp, int8_t* __restrict__ q, const ScaleOut out,
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   }
 }
 
-// Rows longer than the registers of a workgroup: read twice.
+// Rows longer than the registers of a workgroup (16384 columns): read twice.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __restrict__ x, int64_t n_rows, int64_t k,
                                                                  int64_t kp, int8_t* __restrict__ q,
@@ -155,38 +156,29 @@ int launch_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t k, in
                                   : launch_quantize<float>(x, n_rows, k, q, out, clear, s);
 }
 
-// The product for every shape: 64 x 64 tiles, 64 bytes of K staged at a time, four
-// codes a multiply-add (v_dot4).
+// The gate/up product without matrix cores, for what those kernels leave: gathered codes
+// of 4 GiB and more, whose rows 32-bit offsets do not reach. 64 x 64 tiles, 64 bytes of
+// K staged at a time, four codes a multiply-add (v_dot4), which bounds it.
 constexpr int kTile = 64, kStep = 64, kPad = 16;
 
-template <typename T, bool kGateUp>
-__global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
+template <typename T>
+__global__ __launch_bounds__(256) void gate_up_dot4_kernel(const Int8Gemm p) {
   const int tile = blockIdx.x;
-  int e = 0;
-  int64_t row0, rows;
-  if (p.tiles != nullptr) {
-    if (tile >= min(p.tiles[0], (int)min((int64_t)p.tiles[2], p.capacity))) return;
-    const int32_t* ti = p.tiles + ASTRAI_MOE_TILE_HEADER + (int64_t)tile * ASTRAI_MOE_TILE_STRIDE;
-    e = ti[0];
-    row0 = ti[1];
-    rows = min((int64_t)p.tiles[1], (int64_t)ti[2] - row0);
-  } else {
-    row0 = (int64_t)tile * p.block_m;
-    rows = min((int64_t)p.block_m, p.n_rows - row0);
-  }
+  if (tile >= min(p.tiles[0], (int)min((int64_t)p.tiles[2], p.capacity))) return;
+  const int32_t* const ti = p.tiles + ASTRAI_MOE_TILE_HEADER + (int64_t)tile * ASTRAI_MOE_TILE_STRIDE;
+  const int64_t e = ti[0], row0 = ti[1], rows = min(p.tiles[1], ti[2] - ti[1]);
   const int64_t n0 = (int64_t)blockIdx.y * kTile;
-  const int8_t* const w0 = p.w0 + (int64_t)e * p.n * p.kp;
-  const int8_t* const w1 = kGateUp ? p.w1 + (int64_t)e * p.n * p.kp : nullptr;
+  const int8_t* const w0 = p.w0 + e * p.n * p.kp;
+  const int8_t* const w1 = p.w1 + e * p.n * p.kp;
   __shared__ __attribute__((aligned(16))) int8_t As[kTile][kStep + kPad];
   __shared__ __attribute__((aligned(16))) int8_t B0[kTile][kStep + kPad];
-  __shared__ __attribute__((aligned(16))) int8_t B1[kGateUp ? kTile : 1][kStep + kPad];
+  __shared__ __attribute__((aligned(16))) int8_t B1[kTile][kStep + kPad];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int lr = threadIdx.x / 4, lc = threadIdx.x % 4 * 16;  // staged row and byte
   for (int64_t rs = 0; rs < rows; rs += kTile) {
     int acc0[4][4] = {}, acc1[4][4] = {};
-    const int64_t r = row0 + rs + lr;
     const bool row_in = rs + lr < rows, col_in = n0 + lr < p.n;
-    const int64_t src = row_in ? (p.row_src != nullptr ? p.row_src[r] : r) : 0;
+    const int64_t src = row_in ? p.row_src[row0 + rs + lr] : 0;
     for (int64_t k0 = 0; k0 < p.kp; k0 += kStep) {
       const bool k_in = k0 + lc < p.kp;
       const uint4 none = make_uint4(0, 0, 0, 0);
@@ -194,9 +186,8 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
           row_in && k_in ? *reinterpret_cast<const uint4*>(p.a + src * p.kp + k0 + lc) : none;
       *reinterpret_cast<uint4*>(&B0[lr][lc]) =
           col_in && k_in ? *reinterpret_cast<const uint4*>(w0 + (n0 + lr) * p.kp + k0 + lc) : none;
-      if (kGateUp)
-        *reinterpret_cast<uint4*>(&B1[lr][lc]) =
-            col_in && k_in ? *reinterpret_cast<const uint4*>(w1 + (n0 + lr) * p.kp + k0 + lc) : none;
+      *reinterpret_cast<uint4*>(&B1[lr][lc]) =
+          col_in && k_in ? *reinterpret_cast<const uint4*>(w1 + (n0 + lr) * p.kp + k0 + lc) : none;
       __syncthreads();
       for (int kk = 0; kk < kStep; kk += 4) {
         int a[4], b0[4], b1[4];
@@ -205,14 +196,14 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           b0[j] = *reinterpret_cast<const int*>(&B0[tx + 16 * j][kk]);
-          if (kGateUp) b1[j] = *reinterpret_cast<const int*>(&B1[tx + 16 * j][kk]);
+          b1[j] = *reinterpret_cast<const int*>(&B1[tx + 16 * j][kk]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             acc0[i][j] = __builtin_amdgcn_sdot4(a[i], b0[j], acc0[i][j], false);
-            if (kGateUp) acc1[i][j] = __builtin_amdgcn_sdot4(a[i], b1[j], acc1[i][j], false);
+            acc1[i][j] = __builtin_amdgcn_sdot4(a[i], b1[j], acc1[i][j], false);
           }
       }
       __syncthreads();
@@ -227,14 +218,7 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
       for (int j = 0; j < 4; ++j) {
         const int64_t n = n0 + tx + 16 * j;
         if (n >= p.n) continue;
-        const float s0 = p.s0[(int64_t)e * p.n + n];
-        float v;
-        if (kGateUp) {
-          v = swiglu<T>(acc0[i][j], acc1[i][j], sa, s0, p.s1[(int64_t)e * p.n + n]);
-        } else {
-          v = (float)acc0[i][j] * (sa * s0);
-          if (p.bias != nullptr) v += Elem<T>::to_f32(static_cast<const T*>(p.bias)[n]);
-        }
+        const float v = swiglu<T>(acc0[i][j], acc1[i][j], sa, p.s0[e * p.n + n], p.s1[e * p.n + n]);
         static_cast<T*>(p.c)[row * p.n + n] = Elem<T>::from_f32(v);
       }
     }
@@ -242,20 +226,20 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(const Int8Gemm p) {
 }
 
 template <typename T>
-int launch_general(const Int8Gemm& g, hipStream_t s) {
+int launch_gate_up_dot4(const Int8Gemm& g, hipStream_t s) {
   const int64_t cols = ceil_div(g.n, kTile);
   ASTRAI_REQUIRE(g.capacity < (1ll << 31) && cols < 65536, "int8 product: too many tiles");
   if (g.capacity == 0) return ASTRAI_MOE_OK;
-  hipLaunchKernelGGL((g.w1 != nullptr ? gemm_int8_kernel<T, true> : gemm_int8_kernel<T, false>),
-                     dim3((unsigned)g.capacity, (unsigned)cols), dim3(256), 0, s, g);
-  return check_launch("gemm_int8_kernel");
+  hipLaunchKernelGGL((gate_up_dot4_kernel<T>), dim3((unsigned)g.capacity, (unsigned)cols), dim3(256), 0, s, g);
+  return check_launch("gate_up_dot4_kernel");
 }
 
 // out[t] = sum over the routed slots of w y + (sum over the shared ones of y) /
 // n_shared: 32-bit sums in the order of the slots, rounded once. A slot of weight 0
 // adds nothing, whatever its row holds (padding tokens have only such).
 // One workgroup per token (and 2048 columns), a thread per VW columns; the rows' loads
-// of up to 8 slots in flight at a time.
+// of up to 8 slots in flight at a time. Bound by reading y and writing out: 16384 tokens
+// of 2 rows of 4096 bf16 values 96 us (4.2 TB/s).
 template <typename T, int VW>
 __global__ __launch_bounds__(256) void sum_slots_kernel(const T* __restrict__ y, const int32_t* __restrict__ token_pos,
                                                         const T* __restrict__ row_w, int64_t n_tokens, int top_k,
@@ -431,16 +415,15 @@ struct LayerPlan {
 
 }  // namespace
 
+// (gate/up products gather their rows, the others do not)
 int launch_int8_gemm(const Int8Gemm& g, hipStream_t s) {
-  if (g.a == nullptr || (g.w1 != nullptr) == (g.row_src != nullptr) && (g.row_src == nullptr || g.a_bytes < (1ll << 32)))
-    return launch_int8_mfma(g, s);
-  return g.dtype == ASTRAI_MOE_BF16 ? launch_general<bf16_t>(g, s) : launch_general<float>(g, s);
+  if (g.a == nullptr || g.row_src == nullptr || g.a_bytes < (1ll << 32)) return launch_int8_mfma(g, s);
+  return g.dtype == ASTRAI_MOE_BF16 ? launch_gate_up_dot4<bf16_t>(g, s) : launch_gate_up_dot4<float>(g, s);
 }
 
 }  // namespace astrai_moe
 
 using namespace astrai_moe;
-
 
 extern "C" int64_t astrai_moe_int8_row_bytes(int64_t k) { return k < 0 ? -1 : int8_row_bytes(k); }
 

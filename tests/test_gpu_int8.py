@@ -194,6 +194,25 @@ def test_operands_off_16_byte_boundaries(gpu, m, k, n, dtype):
     assert torch.equal(q, want_q) and torch.equal(s, want_s)
 
 
+def test_codes_past_4_gib(gpu):
+    """Rows whose codes lie past 32-bit offsets have the bits that they have alone: a
+    Linear's, which are counted from their tile, and a layer's, which are gathered."""
+    k, m, n = 131072, 2 ** 15 + 70, 40
+    some = torch.tensor([0, 1, 31, 16383, 16384, 2 ** 15 - 1, 2 ** 15, 2 ** 15 + 69], device=gpu)
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=gpu)
+    gen = torch.Generator(gpu).manual_seed(1)
+    for i in range(0, m, 4096):
+        x[i:i + 4096].normal_(generator=gen)
+    w, ws = _weight(gpu, n, k, 2)
+    few = x[some].contiguous()
+    assert torch.equal(ops.int8_linear(x, w, ws)[some], ops.int8_linear(few, w, ws))
+    experts = _experts(gpu, 2, k, 24)
+    logits = torch.randn(m, 2, generator=gen, device=gpu)
+    got = ops.moe_int8_forward(x, logits, experts, 1, routing=ops.Routing("sigmoid"))[some]
+    want = ops.moe_int8_forward(few, logits[some].contiguous(), experts, 1, routing=ops.Routing("sigmoid"))
+    assert torch.equal(got, want)
+
+
 def test_rows_do_not_depend_on_their_company(gpu):
     """Exact sums: a row's bits are the same in every batch, whatever kernel its
     size takes."""
