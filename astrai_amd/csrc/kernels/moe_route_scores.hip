@@ -732,9 +732,12 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
 
 // dlogits of a token from dw, the gradient of its weights, at the chosen experts
 // (a slot of weight 0 has no part: it was filled without a live expert, or its
-// score is below every float):
-//   ds_k = scale (dw_k - sum_j dw_j s_j / S) / S, or scale dw_k
-//   sigmoid: dl = ds s (1 - s);  softmax: dl_e = s_e (ds_e - sum_j ds_j s_j).
+// score is below every float), g_k = scale dw_k:
+//   renormalised, r_k = s_k / S:  dl_k = r_k sum_j r_j (g_k - g_j), sigmoid times 1 - s_k,
+//     and 0 at the others (a softmax over the row and S cancel); of differences, so that
+//     one expert alone, or one that has nearly all the weight, loses no digits
+//   otherwise:  sigmoid dl_k = g_k s_k (1 - s_k), softmax dl_e = s_e (g_e - sum_j g_j s_j).
+// A wave per token, slot k in lane k; columns lane, lane + 64, ... of the row.
 template <typename T, typename W, int ITER>
 __global__ __launch_bounds__(256) void route_scores_grad_kernel(
     const T* __restrict__ logits, const int32_t* __restrict__ topk_idx, const W* __restrict__ topk_w,
@@ -746,49 +749,55 @@ __global__ __launch_bounds__(256) void route_scores_grad_kernel(
   const bool mine = lane < top_k;
   const int idx = mine ? topk_idx[t * top_k + lane] : -1;
   const float wk = mine ? Elem<W>::to_f32(topk_w[t * top_k + lane]) : 0.0f;
-  const float g = mine && wk != 0.0f ? Elem<W>::to_f32(dw[t * top_k + lane]) : 0.0f;
+  const float g = mine && wk != 0.0f ? Elem<W>::to_f32(dw[t * top_k + lane]) * opt.scale : 0.0f;
   const T* const row = logits + t * n_experts;
-  const bool softmax = opt.score == ASTRAI_MOE_SCORE_SOFTMAX;
+  const bool softmax = opt.score == ASTRAI_MOE_SCORE_SOFTMAX, renorm = opt.renormalise != 0;
   const float chosen = idx >= 0 && idx < n_experts && wk != 0.0f ? Elem<T>::to_f32(row[idx]) : -INFINITY;
-  float p[ITER], s = 0.0f, slope = 0.0f;
+  float p[ITER], s = 0.0f, against = 1.0f;  // (against: 1 - s of a sigmoid)
   if (softmax) {
-    float mx = -INFINITY;
+    float mx = chosen;
+    if (!renorm)
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      const int c = lane + i * 64;
-      p[i] = c < n_experts ? Elem<T>::to_f32(row[c]) : -INFINITY;
-      mx = fmaxf(mx, p[i]);
-    }
+      for (int i = 0; i < ITER; ++i) {
+        const int c = lane + i * 64;
+        p[i] = c < n_experts ? Elem<T>::to_f32(row[c]) : -INFINITY;
+        mx = fmaxf(mx, p[i]);
+      }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
     if (mx == -INFINITY) mx = 0.0f;
-    float sum = 0.0f;
+    s = expf(chosen - mx);
+    if (!renorm) {
+      float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      p[i] = expf(p[i] - mx);
-      sum += p[i];
+      for (int i = 0; i < ITER; ++i) {
+        p[i] = expf(p[i] - mx);
+        sum += p[i];
+      }
+      sum = wave_sum(sum);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) p[i] *= inv;
+      s *= inv;
     }
-    sum = wave_sum(sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) p[i] *= inv;
-    s = expf(chosen - mx) * inv;
   } else {
-    // s (1 - s) = s(l) s(-l), without the cancellation of 1 - s
+    // 1 - s(l) = s(-l), without the cancellation
     const float e = expf(-fabsf(chosen)), d = 1.0f / (1.0f + e);
     s = chosen >= 0.0f ? d : e * d;
-    slope = e * d * d;
+    against = chosen >= 0.0f ? e * d : d;
   }
-  const float S = wave_sum(s);
-  float ds = g * opt.scale;
-  if (opt.renormalise) {
-    const float inv = S == 0.0f ? 0.0f : 1.0f / S;
-    const float dot = wave_sum(ds * s) * inv;
-    ds = wk != 0.0f ? (ds - dot) * inv : 0.0f;
+  float at_chosen, dot = 0.0f;
+  if (renorm) {
+    const float S = wave_sum(s), r = S == 0.0f ? 0.0f : s / S;
+    float sum = 0.0f;
+    for (int k = 0; k < top_k; ++k) sum += __shfl(r, k, 64) * (g - __shfl(g, k, 64));
+    at_chosen = r * sum * against;
+  } else {
+    at_chosen = softmax ? g : g * s * against;
+    if (softmax) dot = wave_sum(g * s);
   }
-  if (wk != wk) ds = wk;
-  const float at_chosen = softmax ? ds : ds * slope;
-  const float dot = softmax ? wave_sum(ds * s) : 0.0f;
+  if (wk != wk) at_chosen = wk;  // (the row holds no number)
+  const bool poison = softmax && __any(wk != wk);
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int c = lane + i * 64;
@@ -798,7 +807,8 @@ __global__ __launch_bounds__(256) void route_scores_grad_kernel(
       const float v = __shfl(at_chosen, k, 64);
       if (e == c) d = v;
     }
-    if (c < n_experts) dlogits[t * n_experts + c] = Elem<T>::from_f32(softmax ? p[i] * (d - dot) : d);
+    if (softmax && !renorm) d = p[i] * (d - dot);
+    if (c < n_experts) dlogits[t * n_experts + c] = Elem<T>::from_f32(poison ? NAN : d);
   }
 }
 

@@ -161,6 +161,38 @@ def test_route_scores_grad(gpu, t, e, k, routing, dtype, weight_dtype, masked):
     assert (err <= (REL + HALF[dtype]) * ref.abs() + 2.0 ** -16 * size).all(), (err - HALF[dtype] * ref.abs()).max()
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_gradient_of_weights_that_cannot_change(gpu, score):
+    """Renormalised, the weight of one expert alone is constant: no gradient, not a
+    rounding's worth. The same where the others are off, and for equal dw; and of a
+    softmax nothing at the experts that were not chosen."""
+    logits, _ = _inputs(gpu, 300, 384, torch.float32, False, False)
+    dw = torch.randn(300, 4, generator=torch.Generator().manual_seed(2)).to(gpu)
+    for k, lo in ((1, logits), (3, logits.masked_fill(torch.arange(384, device=gpu) != 5, -math.inf))):
+        r = ops.moe_route_scores(lo, k, ops.Routing(score, scale=2.5))
+        assert (ops.moe_route_scores_grad(lo, r.topk_idx, r.topk_w, dw[:, :k].contiguous(), ops.Routing(score, scale=2.5)) == 0).all()
+    r = ops.moe_route_scores(logits, 4, ops.Routing(score))
+    assert (ops.moe_route_scores_grad(logits, r.topk_idx, r.topk_w, dw[:, :1].expand(-1, 4).contiguous(), ops.Routing(score)) == 0).all()
+    got = ops.moe_route_scores_grad(logits, r.topk_idx, r.topk_w, dw, ops.Routing(score))
+    assert (got.scatter(1, r.topk_idx.long(), 0.0) == 0).all() and (got != 0).any(1).all()
+
+
+def test_gradient_of_a_weight_near_one(gpu):
+    """One expert far above the others: its gradient is small, and keeps its digits
+    (every factor of the formula in differences within 2^-17 of its own size)."""
+    logits, _ = _inputs(gpu, 200, 64, torch.float32, False, False)
+    logits[:, 7] = 25.0
+    dw = torch.randn(200, 4, generator=torch.Generator().manual_seed(2)).to(gpu)
+    routing = ops.Routing("softmax")
+    r = ops.moe_route_scores(logits, 4, routing)
+    got = ops.moe_route_scores_grad(logits, r.topk_idx, r.topk_w, dw, routing)
+    w = torch.softmax(logits.double().gather(1, r.topk_idx.long()), -1)
+    terms = w.unsqueeze(2) * w.unsqueeze(1) * (dw.double().unsqueeze(2) - dw.double().unsqueeze(1))
+    want = terms.sum(2)
+    err = (got.gather(1, r.topk_idx.long()).double() - want).abs()
+    assert (err <= 2.0 ** -17 * terms.abs().sum(2)).all()
+
+
 def test_gradient_against_differences(gpu):
     """dw . d(weights) along random directions, by central differences of the
     64-bit weights at the kernel's choice."""
