@@ -17,6 +17,7 @@
 #include "mfma_pick.h"
 #include "mfma_tile.h"
 #include "moe_int8.h"
+#include "wave_lanes.h"
 
 #include <type_traits>
 
@@ -39,19 +40,19 @@ struct RowTiles {
   const int32_t* tiles;
   int n_rows, block_m;
   __device__ int live(int capacity) const {
-    return tiles == nullptr ? capacity : min(tiles[0], min(tiles[2], capacity));
+    return tiles == nullptr ? capacity : min(load_scalar(tiles), min(load_scalar(tiles + 2), capacity));
   }
-  __device__ int height() const { return tiles == nullptr ? block_m : tiles[1]; }
+  __device__ int height() const { return tiles == nullptr ? block_m : load_scalar(tiles + 1); }
   __device__ void get(int mt, int& e, int& row0, int& end) const {
     if (tiles == nullptr) {
       e = 0;
       row0 = mt * block_m;
       end = n_rows;
     } else {
-      const int32_t* ti = tiles + ASTRAI_MOE_TILE_HEADER + (int64_t)mt * ASTRAI_MOE_TILE_STRIDE;
-      e = ti[0];
-      row0 = ti[1];
-      end = ti[2];
+      const int32_t* ti = tiles + ASTRAI_MOE_TILE_HEADER + (int64_t)uniform(mt) * ASTRAI_MOE_TILE_STRIDE;
+      e = load_scalar(ti);
+      row0 = load_scalar(ti + 1);
+      end = load_scalar(ti + 2);
     }
   }
 };
@@ -64,9 +65,8 @@ struct Args {
   const int8_t *w0, *w1;
   const float *s0, *s1;
   const void* bias;
-  const void* x;  // rows to quantise in the kernel, their columns, and whether they are aligned to 16 bytes
+  const void* x;  // rows to quantise in the kernel, and their columns
   int64_t k;
-  bool vec;
   int kp, n, n_tiles_n, capacity;
   void* c;
   float* part;     // partial sums of a split last round, or null
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(StreamCfg<kGateUp>::THREADS, 1) void gemm_i8_stream
   // Waves of padding rows only idle where gemm_stream_kernel's do.
   const int idle_row0 = __builtin_amdgcn_readfirstlane(wm * Cfg::WM);
   const int idle_mt0 =
-      __builtin_amdgcn_readfirstlane(KT < kIdleMaxSteps || p.tiles.tiles == nullptr ? 0 : p.tiles.tiles[3]);
+      __builtin_amdgcn_readfirstlane(KT < kIdleMaxSteps || p.tiles.tiles == nullptr ? 0 : load_scalar(p.tiles.tiles + 3));
   walk.item(seq.id(0), mt, nt, k0, k1, unit);
   for (int idx = 0;; ++idx) {
     const int claim_at = (claiming && seq.claims_next(idx)) ? k1 - kClaimLead : -1;
@@ -970,9 +970,10 @@ __global__ __launch_bounds__(Cfg::WAVES * 64, 1) void gemm_i8_few_kernel(const A
 // most 16) rows of its row tile, whose codes stay in LDS, behind its first weight
 // loads: for one token the launch and the trip through memory that a quantiser of its
 // own takes (4 to 5 us) are most of a small product's time. Otherwise as above. The rows
-// are held in two units of 512 values a wave (UNITS), where it breaks even (us a product,
-// so / with a quantiser: 4096 to 14336, 1 row 17 / 20; 2048 x 2 rows 8.6 / 8.2; 1024 x 4
-// 6.5 / 7.0, x 8 8.7 / 7.0; 512 x 4 5.2 / 5.9, x 8 6.4 / 5.9).
+// are held in two units of 512 values a wave (UNITS); a third and fourth cost 1.2 to 1.7
+// us, as much as a quantiser of its own or more (us a product with them / a quantiser:
+// 4096 to 14336, 2 rows 20.2 / 19.0; 2048 to 5632, 4 rows 9.3 / 7.8; 1024 to 4096, 8 rows
+// 7.8 / 7.3; of two units 4096 to 14336, 1 row 18.4, 2048 to 5632 6.6, 512 to 1536 4.3).
 // ===========================================================================
 struct QuantCfg {
   static constexpr int BM = 16, BN = 32, WAVES = 4, STAGES = 8, UNITS = 2;
@@ -984,7 +985,7 @@ struct QuantCfg {
   static_assert(LDS + 256 <= 160 * 1024, "LDS");
 };
 
-template <typename T, bool kGateUp, bool kGather>
+template <typename T, bool kGateUp, bool kGather, bool kVec>
 __global__ __launch_bounds__(QuantCfg::WAVES * 64, 1) void gemm_i8_quant_kernel(const Args p) {
   using Cfg = QuantCfg;
   using C = typename CodeType<T>::type;
@@ -1057,33 +1058,28 @@ __global__ __launch_bounds__(QuantCfg::WAVES * 64, 1) void gemm_i8_quant_kernel(
     unit_row[i] = (wave + 4 * i) / chunks;
     unit_col[i] = (wave + 4 * i - unit_row[i] * chunks) * 512 + lane * 8;
   }
+  // (a unit without a row loads the first one's again)
   auto load_rows = [&](int row0, int rows) {
 #pragma unroll
     for (int i = 0; i < Cfg::UNITS; ++i) {
-      const int r = unit_row[i], col = unit_col[i];
-      if (r >= rows) break;
+      const int r = unit_row[i] < rows ? unit_row[i] : 0;
       const int64_t src = kGather ? p.row_src[row0 + r] : row0 + r;
-      const T* const row = static_cast<const T*>(p.x) + src * p.k;
-      if (p.vec)
-        v[i].template load<true>(row, col, p.k);
-      else
-        v[i].template load<false>(row, col, p.k);
+      v[i].template load<kVec>(static_cast<const T*>(p.x) + src * p.k, unit_col[i], p.k);
     }
   };
-  // (after a barrier behind the last reads of the tile before) the rows' codes and maxima
+  // (after a barrier behind the last reads of the tile before) the rows' codes and maxima.
+  // Every unit's load is used: one left in flight would have the loop below wait for all.
   auto quantise = [&](int rows) {
     if (threadIdx.x < Cfg::BM) s_top[threadIdx.x] = 0;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int i = 0; i < Cfg::UNITS; ++i) {
       const int r = unit_row[i];
-      if (r >= rows) break;
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, v[i].bits(j) & 0x7fffffffu);
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-      if (lane == 0) atomicMax(&s_top[r], top);
+      top = lanes_max<64>(top);
+      if (lane == 0 && r < rows) atomicMax(&s_top[r], top);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
@@ -1202,7 +1198,6 @@ Args args_of(const Int8Gemm& g) {
   a.tiles = RowTiles{g.tiles, (int)g.n_rows, g.block_m};
   a.w0 = g.w0, a.w1 = g.w1, a.s0 = g.s0, a.s1 = g.s1, a.bias = g.bias;
   a.x = g.x, a.k = g.k;
-  a.vec = g.k * (g.dtype == ASTRAI_MOE_BF16 ? 2 : 4) % 16 == 0 && aligned16(g.x);
   a.kp = (int)g.kp, a.n = (int)g.n, a.capacity = (int)g.capacity, a.c = g.c;
   return a;
 }
@@ -1308,7 +1303,9 @@ int launch_quant(const Int8Gemm& g, hipStream_t s) {
   a.n_tiles_n = (int)n_cols;
   int64_t grid = 0;
   if (int rc = persistent_grid(g.capacity, n_cols, &grid)) return rc;
-  hipLaunchKernelGGL((gemm_i8_quant_kernel<T, kGateUp, kGather>), dim3((unsigned)grid), dim3(QuantCfg::WAVES * 64), 0, s, a);
+  const bool vec = g.k * (int64_t)sizeof(T) % 16 == 0 && aligned16(g.x);  // (the rows' 16-byte pieces)
+  hipLaunchKernelGGL((vec ? gemm_i8_quant_kernel<T, kGateUp, kGather, true> : gemm_i8_quant_kernel<T, kGateUp, kGather, false>),
+                     dim3((unsigned)grid), dim3(QuantCfg::WAVES * 64), 0, s, a);
   return check_launch(kGateUp ? "gemm_i8_quant_kernel<gate_up>" : "gemm_i8_quant_kernel<down>");
 }
 #endif

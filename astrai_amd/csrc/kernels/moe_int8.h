@@ -97,13 +97,18 @@ template <typename T>
 struct Unit {
   static constexpr int WORDS = 2 * sizeof(T);
   uint32_t w[WORDS];
-  // from column c on, zeros from column k on; kVec: 16-byte loads (aligned rows)
+  // from column c on, zeros from column k on; kVec: 16-byte loads (rows of whole 16-byte
+  // pieces on 16-byte boundaries), without a branch, so that several are in flight
   template <bool kVec>
   __device__ __forceinline__ void load(const T* row, int64_t c, int64_t k) {
-    if (kVec && c + 8 <= k) {
+    if (kVec) {
 #pragma unroll
-      for (int j = 0; j < WORDS; j += 4)
-        *reinterpret_cast<uint4*>(&w[j]) = *reinterpret_cast<const uint4*>(row + c + j * (4 / (int)sizeof(T)));
+      for (int j = 0; j < WORDS; j += 4) {
+        const int64_t at = c + j * (4 / (int)sizeof(T));
+        const bool in = at < k;
+        const uint4 v = *reinterpret_cast<const uint4*>(row + (in ? at : 0));
+        w[j] = in ? v.x : 0, w[j + 1] = in ? v.y : 0, w[j + 2] = in ? v.z : 0, w[j + 3] = in ? v.w : 0;
+      }
     } else {
       T in[8];
 #pragma unroll

@@ -14,6 +14,7 @@
 // middle between two codes, as x = max / 2 always is, must not turn on a last bit.
 #include "moe_common.h"
 #include "moe_int8.h"
+#include "wave_lanes.h"
 
 namespace astrai_moe {
 namespace {
@@ -60,8 +61,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, v[i].bits(j) & 0x7fffffffu);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  top = lanes_max<64>(top);
   if constexpr (WAVES > 1) {
     if (lane == 0) s_most[wave] = __uint_as_float(top);
     __syncthreads();
@@ -96,8 +96,7 @@ __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const T* __rest
   const T* const row = x + r * k;
   uint32_t top = 0;
   for (int64_t c = threadIdx.x; c < k; c += 256) top = max(top, __float_as_uint(Elem<T>::to_f32(row[c])) & 0x7fffffffu);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  top = lanes_max<64>(top);
   if (lane == 0) s_top[wave] = top;
   __syncthreads();
   top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
