@@ -78,6 +78,8 @@ class ScoredMoE(DeepSeekMoE):
         topk_w, topk_idx, chunk_hist = ScoredRouteWeights.apply(logits, self.balance_bias, self.n_activated_experts,
                                                                 self.routing, dtype)
         if self.track_load and self.training:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("track_load: a captured graph's replays would not be counted; capture with track_load off")
             load = ops.moe_expert_load(chunk_hist)
             self.load = load if self.load is None else self.load.add_(load)
         return topk_w, topk_idx, chunk_hist
@@ -88,10 +90,13 @@ class ScoredMoE(DeepSeekMoE):
         tokens than the mean since the last call and down for those that got
         more; returns the loads it went by (None, and no change, without
         tracked forwards). ``group``: a process group over whose ranks the
-        loads are summed first (``torch.distributed.group.WORLD`` for all)."""
+        loads are summed first (``torch.distributed.group.WORLD`` for all);
+        every rank of it calls, also one that tracked no forward."""
         load, self.load = self.load, None
         if load is None:
-            return None
+            if group is None:
+                return None
+            load = torch.zeros(self.balance_bias.shape, dtype=torch.int32, device=self.balance_bias.device)
         if group is not None:
             if torch.distributed.get_backend(group) == "gloo":  # (sums host tensors)
                 host = load.cpu()

@@ -303,3 +303,31 @@ def test_balance_sums_over_a_gloo_group(gpu):
         assert load.sum().item() == 200
     finally:
         dist.destroy_process_group()
+
+
+def test_balance_of_a_rank_without_tracked_forwards(gpu):
+    """Alone there is nothing to do; of a group it takes part, with no loads."""
+    import torch.distributed as dist
+
+    layer = _layer(gpu, torch.float32, track_load=True, **GROUPED)
+    before = layer.balance_bias.clone()
+    assert layer.update_balance(0.01) is None
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        assert (layer.update_balance(0.01, group=dist.group.WORLD) == 0).all()
+    finally:
+        dist.destroy_process_group()
+    assert torch.equal(layer.balance_bias, before)
+
+
+def test_tracked_forwards_are_not_captured(gpu):
+    layer = _layer(gpu, torch.float32, track_load=True, **GROUPED)
+    x = torch.randn(1, 50, 256, device=gpu)
+    layer(x)
+    layer.update_balance(0.01)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="track_load"):
+        with torch.cuda.graph(graph):
+            layer(x)
+    layer(x)
+    assert layer.load.sum().item() == 200
