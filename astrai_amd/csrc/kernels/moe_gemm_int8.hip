@@ -451,13 +451,12 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void gemm_i8_kernel(const Args p) 
 // gemm_stream_kernel of moe_gemm_mfma.hip, whose comments give the reasons of its
 // schedule: two activation and three weight stages, one barrier a K step, the
 // matrix-core waves' fragments in rings, the priority drops. 16384 tokens, 8 experts,
-// top-2, D 4096, F 14336: gate/up 2.90 to 3.04 ms (2.5 to 2.65 Pop/s), down 1.32 to 1.40
-// (2.75 to 2.9); one expert, 8192 rows, 4096 to 14336 364 to 427 us (2.25 to 2.64). A
-// K step of a tile takes 1.54 us, of which the matrix instructions alone, with their
+// top-2, D 4096, F 14336: gate/up 2.73 to 2.86 ms (2.7 to 2.8 Pop/s), down 1.34 to 1.43
+// (2.7 to 2.9); one expert, 8192 rows, 4096 to 14336 364 to 443 us (2.2 to 2.64). A K
+// step of a tile takes about 1.46 us, of which the matrix instructions alone, with their
 // operands in registers on every compute unit at once, take 1.07 (4.0 Pop/s; those of
-// 32 x 32 x 32 3.5); a tile's epilogue and first fragments take 5 us, the tenth by
-// which the shorter K of the gate/up product falls behind (matrix cores busy 73%, down
-// 85%).
+// 32 x 32 x 32 3.5); a tile's epilogue and first fragments take about 3 us, of which the
+// gate/up product's shorter K has more (matrix cores busy 79%, down 83%).
 // ===========================================================================
 template <bool kGateUp>
 struct StreamCfg {

@@ -561,8 +561,9 @@ int astrai_moe_route_scores(const void* logits, int dtype, const float* bias,
 
 /*
  * Gradient of the logits from dw, that of astrai_moe_route_scores' weights, at
- * the chosen experts, in float with one rounding to dtype. Slots of weight 0 have
- * no part in it; the bias gets no gradient (it moves the choice only).
+ * the chosen experts (a softmax that is not renormalised: at all), in float with one
+ * rounding to dtype. Slots of weight 0 have no part in it; the bias gets no gradient
+ * (it moves the choice only).
  *   topk_idx, topk_w  as astrai_moe_route_scores wrote them
  *   dw                [n_tokens, top_k]      weight_dtype
  *   dlogits           [n_tokens, n_experts]  dtype
@@ -630,7 +631,7 @@ int astrai_moe_quantize_rows(const void* x, int dtype, int64_t n_rows,
  *   workspace  astrai_moe_int8_linear_workspace_bytes(...) bytes for the same
  *              sizes, 256-byte aligned, nothing to initialise; calls sharing one
  *              must not overlap
- *   out        [n_rows, n]              dtype
+ *   out        [n_rows, n]              dtype, apart from x
  */
 int64_t astrai_moe_int8_linear_workspace_bytes(int64_t n_rows, int64_t k,
                                                int64_t n, int dtype);
