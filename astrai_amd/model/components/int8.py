@@ -57,6 +57,8 @@ class Int8Linear(nn.Module):
 
     def forward(self, x: Tensor) -> Tensor:
         _check_input(x, "Int8Linear")
+        if x.shape[-1] != self.in_dim:  # (rows of codes are padded: their bytes do not tell)
+            raise ValueError(f"Int8Linear of {self.in_dim} columns got {x.shape[-1]}")
         lead = x.shape[:-1]
         bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
         out = ops.int8_linear(x.reshape(-1, x.shape[-1]).contiguous(), self.weight, self.weight_scale, bias)

@@ -69,6 +69,8 @@ class ScoredMoE(DeepSeekMoE):
 
     def _apply(self, *args, **kwargs):
         keep_float32(self, ("balance_bias",), super()._apply, *args, **kwargs)
+        if self.load is not None:
+            self.load = self.load.to(self.balance_bias.device)
         return self
 
     def _routing(self) -> tuple[ops.Routing, Tensor]:

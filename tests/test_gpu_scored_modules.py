@@ -331,3 +331,11 @@ def test_tracked_forwards_are_not_captured(gpu):
             layer(x)
     layer(x)
     assert layer.load.sum().item() == 200
+
+
+def test_int8_linear_knows_its_columns(gpu):
+    """97 and 100 columns take the same bytes of codes."""
+    lin = Int8Linear.from_linear(torch.nn.Linear(100, 24, bias=False).to(gpu))
+    assert lin(torch.randn(3, 100, device=gpu)).shape == (3, 24)
+    with pytest.raises(ValueError, match="columns"):
+        lin(torch.randn(3, 97, device=gpu))
