@@ -748,7 +748,7 @@ __global__ __launch_bounds__(256) void route_scores_grad_kernel(
     for (int k = 0; k < top_k; ++k) {
       const int e = __shfl(idx, k, 64);
       const float v = __shfl(at_chosen, k, 64);
-      if (e == c) d = v;
+      if (e == c) d += v;
     }
     if (softmax && !renorm) d = p[i] * (d - dot);
     if (c < n_experts) dlogits[t * n_experts + c] = Elem<T>::from_f32(poison ? NAN : d);
@@ -813,15 +813,19 @@ int launch_scores(const void* logits, const float* bias, const astrai_moe_routin
 #define ROUTE_CASE(L, C)                                                                                       \
   launch_scores_cfg<T, W, L, C>(logits, bias, opt, n_tokens, n_experts, top_k, n_shared, topk_idx, topk_w,      \
                                 chunk_hist, list, s)
-  if (n_experts <= 32)
+  // As many lanes as groups, more than 64 of which are for choose_slowly. (16384 tokens, us,
+  // 128 experts in 32 groups by 16 lanes, so choose_slowly, 82, by 32 lanes 32; 256 in 64
+  // groups by 16 lanes 126, by 64 lanes 94.)
+  const bool few = opt.n_groups <= 16;
+  if (n_experts <= 32 && few)
     ROUTE_CASE(16, 2);
-  else if (n_experts <= 64)
+  else if (n_experts <= 64 && few)
     ROUTE_CASE(16, 4);
-  else if (n_experts <= 128)
+  else if (n_experts <= 128 && few)
     ROUTE_CASE(16, 8);
-  else if (n_experts <= 256)
+  else if (n_experts <= 256 && few)
     ROUTE_CASE(16, 16);
-  else if (n_experts <= 512)
+  else if (n_experts <= 512 && opt.n_groups <= 32)
     ROUTE_CASE(32, 16);
   else
     ROUTE_CASE(64, ASTRAI_MOE_MAX_EXPERTS / 64);

@@ -535,8 +535,9 @@ int astrai_moe_gemm_wgrad(const void* a, const void* b,
  *     chosen and weight 0
  *   topk_w = scale s / S over the chosen s, S their sum (0 where S = 0), or with
  *     renormalise 0 scale s; rounded once to weight_dtype
- * The choice is made in 64 bits. A row with a NaN logit (softmax: or +inf) has
- * experts 0 .. top_k - 1 and NaN weights.
+ * Without a bias, c is ordered as its logits are (also where scores in 64 bits are
+ * equal); with one, and for group values of two scores, in 64 bits. A row with a NaN
+ * logit (softmax: or +inf) has experts 0 .. top_k - 1 and NaN weights.
  *
  *   logits     [n_tokens, n_experts]  dtype
  *   bias       [n_experts]            float, or NULL

@@ -303,6 +303,23 @@ def test_logits_that_differ_in_their_last_bits(gpu, score):
         _check_route(ops.moe_route_scores(logits, 6, routing), logits, 6, routing, None, torch.float32)
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_logits_at_the_ends_of_their_range(gpu, score):
+    """Masks of the lowest float and scores that are 0 or 1 in 64 bits: the order of the
+    logits, weight 0 where the score is 0."""
+    for dtype in (torch.float32, torch.bfloat16):
+        low = torch.finfo(dtype).min
+        logits = torch.full((4, 64), low, dtype=dtype, device=gpu)
+        logits[0, 9] = logits[0, 3] = 0.5
+        logits[1, 40], logits[1, 7] = -800.0, -900.0
+        logits[2, 5], logits[2, 6] = 60.0, 62.0
+        r = ops.moe_route_scores(logits, 3, ops.Routing(score))
+        assert r.topk_idx.tolist() == [[3, 9, 0], [40, 7, 0], [6, 5, 0], [0, 1, 2]]
+        assert torch.isfinite(r.topk_w).all() and (r.topk_w[0, :2] == 0.5).all() and (r.topk_w[0, 2] == 0).all()
+        g = ops.moe_route_scores_grad(logits, r.topk_idx, r.topk_w, torch.ones_like(r.topk_w), ops.Routing(score))
+        assert (g == 0).all()
+
+
 def test_large_biases_that_cancel_in_a_group(gpu):
     """Group values whose parts are far larger than their sums: rounded in 32 bits they
     lose what tells the groups apart."""
