@@ -103,7 +103,8 @@ struct TokenLds {
 // Score of one expert in 64 bits (softmax: with the row's maximum and sum).
 __device__ __forceinline__ double score_of(double l, bool softmax, double mx, double sum) {
   if (l == -INFINITY) return 0.0;
-  return softmax ? exp(l - mx) / sum : 1.0 / (1.0 + exp(-l));
+  const double t = exp(softmax ? l - mx : -l);
+  return (softmax ? t : 1.0) / (softmax ? sum : 1.0 + t);
 }
 
 // The choice of one token by a whole wave in 64 bits, for any logits and biases:
@@ -273,12 +274,13 @@ __device__ __forceinline__ uint64_t groups_kept(const float (&value)[C], float t
   const uint64_t kept = best_groups<L>(mine, g, p, opt.topk_groups, last, next);
   if (tol == 0.0f) return kept;
   const float size = lanes_max<L>(mine > -INFINITY ? fabsf(a1) + (two ? fabsf(a2) : 0.0f) : 0.0f);
-  if (__ballot(on && next > -INFINITY && last - next <= 2.0f * tol + 4.0f * kTolAdd * size) == 0) return kept;
+  const bool close = on && next > -INFINITY && last - next <= 2.0f * tol + 4.0f * kTolAdd * size;
+  if (__ballot(close) == 0) return kept;
   const double sum = sum64();
   store();
   const float least = two ? a2 : a1;
   double d1 = -INFINITY, d2 = -INFINITY;
-  for (int j = begin;;) {
+  for (int j = close ? begin : per;;) {
     for (; j < per; j += p) {
       const float v = values[g * per + j];
       if (v > -INFINITY && least - v <= tol + kTolAdd * (fabsf(v) + fabsf(least))) break;
@@ -291,7 +293,8 @@ __device__ __forceinline__ uint64_t groups_kept(const float (&value)[C], float t
   }
   for (int off = 1; off < p; off *= 2) merge_two(d1, d2, __shfl_xor(d1, off, L), __shfl_xor(d2, off, L));
   double last64, next64;
-  return best_groups<L>(two ? d1 + d2 : d1, g, p, opt.topk_groups, last64, next64);
+  const uint64_t exactly = best_groups<L>(two ? d1 + d2 : d1, g, p, opt.topk_groups, last64, next64);
+  return close ? exactly : kept;
 }
 
 // Which of the lane's C experts are in a group that stays, as bits.
@@ -402,31 +405,45 @@ __device__ __forceinline__ float pick(uint32_t (&v)[C], int sub, int top_k, Lds&
 }
 
 // The same from the exact values of the experts that may be chosen (`open`, bits of the
-// lane's), for the few tokens that need them.
+// lane's; none of tokens whose choice stands): each takes the place that the number of
+// better ones gives it. False for a token of more than the list holds.
 template <int L, int C, typename Lds, typename Exact>
-__device__ __forceinline__ void pick_exact(uint32_t open, int sub, int top_k, Lds& m, Exact exact) {
+__device__ __forceinline__ bool pick_exact(uint32_t open, int sub, int top_k, Lds& m, Exact exact) {
+  constexpr int kMost = ASTRAI_MOE_MAX_TOPK, MINE = kMost > L ? kMost / L : 1;
+  int& count = *reinterpret_cast<int*>(m.kept);
+  if (sub == 0) count = 0;
+  wave_sync();
 #pragma unroll 1
-  for (uint32_t left = open; __ballot(left != 0) != 0; left &= left - 1)
-    if (left != 0) {
-      const int e = sub * C + __builtin_ctz(left);
-      m.key[e] = order_of(exact(e));
+  for (; __ballot(open != 0) != 0; open &= open - 1)
+    if (open != 0) {
+      const int e = sub * C + __builtin_ctz(open), at = atomicAdd(&count, 1);
+      const uint64_t v = order_of(exact(e));
+      if (at < kMost) m.key[at] = v, m.pick[at] = e;
     }
-#pragma unroll 1
-  for (int k = 0; k < top_k; ++k) {
-    uint64_t best = kNone;
-    int at = 0;
-#pragma unroll 1
-    for (uint32_t left = open; left != 0; left &= left - 1) {
-      const int i = __builtin_ctz(left);
-      if (m.key[sub * C + i] > best) best = m.key[sub * C + i], at = i;
-    }
-    const uint64_t top = lanes_max<L>(best);
-    if (sub == first_lane<L>(best == top) && top != kNone) {
-      m.pick[k] = sub * C + at;
-      m.score[k] = (float)value_of(top);
-      open &= ~(1u << at);
-    }
+  wave_sync();
+  const int n = count;
+  uint64_t v[MINE];
+  int e[MINE], better[MINE];
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int c = min(sub + i * L, kMost - 1);
+    v[i] = m.key[c], e[i] = m.pick[c], better[i] = 0;
   }
+#pragma unroll 1
+  for (int j = 0; j < min(n, kMost); ++j) {
+    const uint64_t vj = m.key[j];
+    const int ej = m.pick[j];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) better[i] += vj > v[i] || (vj == v[i] && ej < e[i]);
+  }
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < MINE; ++i)
+    if (sub + i * L < n && n <= kMost && better[i] < top_k) {
+      m.pick[better[i]] = e[i];
+      m.score[better[i]] = (float)value_of(v[i]);
+    }
+  return n <= kMost;
 }
 
 // The lane's C of a row of n values from column c0 on, `none` behind its end. vec: rows
@@ -616,9 +633,10 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
           if (sub * C + i < n_experts && (ki >= k0 || beside)) open |= 1u << i;
           close |= beside && left && (l[i] != l0 || b[i] != b0) && swapped(v0, value[i]);
         }
-        if (__ballot(close && on) != 0) {  // (the wave's other tokens get the choice that they have)
+        const bool again = lanes_of<L>(close && on) != 0;
+        if (__ballot(again) != 0) {
           const double sum = bias != nullptr ? sum64() : 0.0;
-          pick_exact<L, C>(open, sub, top_k, m, [&](int e) {
+          odd |= !pick_exact<L, C>(again ? open : 0u, sub, top_k, m, [&](int e) {
             return (in >> (e - sub * C) & 1) == 0 ? -INFINITY
                    : bias != nullptr              ? exact(e, sum)
                                                   : (double)Elem<T>::to_f32(row[e]);
