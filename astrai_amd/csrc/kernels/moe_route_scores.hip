@@ -100,10 +100,14 @@ struct TokenLds {
   uint32_t kept[(E + 31) / 32];
 };
 
+// exp in 64 bits, a call: where it is needed few waves come, and inlined its registers
+// and its code would cost the others theirs.
+__device__ __attribute__((noinline)) double exp64(double x) { return exp(x); }
+
 // Score of one expert in 64 bits (softmax: with the row's maximum and sum).
 __device__ __forceinline__ double score_of(double l, bool softmax, double mx, double sum) {
   if (l == -INFINITY) return 0.0;
-  const double t = exp(softmax ? l - mx : -l);
+  const double t = exp64(softmax ? l - mx : -l);
   return (softmax ? t : 1.0) / (softmax ? sum : 1.0 + t);
 }
 
@@ -349,10 +353,13 @@ __device__ __forceinline__ void sort_down(uint32_t (&v)[C]) {
 
 // Whether the lane's group stays, where groups are 2^shift whole lanes, from what the
 // experts go by (-inf: off): logits, whose `score` groups of two go by, or scores with
-// their biases (scored). `close`: the border lies between two that are near.
-template <int L, int C, typename Score>
+// their biases (scored). Where the border of a token lies between two groups that are
+// near, from exact(expert, sum64()) of the experts that may be a group's best.
+template <int L, int C, typename Lds, typename Score, typename Sum, typename Exact>
 __device__ __forceinline__ bool group_stays(const float (&value)[C], float tol, bool scored, int sub,
-                                            const astrai_moe_routing& opt, int shift, Score score, bool& close) {
+                                            const astrai_moe_routing& opt, int shift, bool on, Lds& m, Score score,
+                                            Sum sum64, Exact exact) {
+  const bool two = opt.group_top == 2;
   float a1 = value[0], a2 = -INFINITY;
 #pragma unroll
   for (int i = 1; i < C; ++i) {
@@ -365,8 +372,9 @@ __device__ __forceinline__ bool group_stays(const float (&value)[C], float tol, 
   if (shift > 3) merge_two(a1, a2, other<3>(a1), other<3>(a2));
   if constexpr (L >= 64)
     if (shift > 4) merge_two(a1, a2, other<4>(a1), other<4>(a2));
+  const float least = two ? a2 : a1;
   float size = fabsf(a1);  // (what the sums' roundings are relative to)
-  if (opt.group_top == 2) {
+  if (two) {
     const float s1 = scored || a1 == -INFINITY ? a1 : score(a1), s2 = scored || a2 == -INFINITY ? a2 : score(a2);
     size = fabsf(s1) + fabsf(s2);
     a1 = s1 + s2;
@@ -379,11 +387,33 @@ __device__ __forceinline__ bool group_stays(const float (&value)[C], float tol, 
     const int at = first_lane<L>(mine == last);
     if (sub >> shift == at >> shift) mine = 0, stays = true;
   }
-  if (tol > 0.0f) {
-    const float next = float_of(max(lanes_max<L>(mine), bits_of(-INFINITY)));
-    close = next > -INFINITY && float_of(last) - next <= 2.0f * tol + 4.0f * kTolAdd * lanes_max<L>(size);
-  }
-  return stays;
+  if (tol == 0.0f) return stays;
+  const float next = float_of(max(lanes_max<L>(mine), bits_of(-INFINITY)));
+  const bool close = on && next > -INFINITY && float_of(last) - next <= 2.0f * tol + 4.0f * kTolAdd * lanes_max<L>(size);
+  if (__ballot(close) == 0) return stays;
+  const double sum = sum64();
+  uint32_t open = 0;  // (logits are exact)
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (value[i] > -INFINITY && least - value[i] <= (scored ? tol + kTolAdd * (fabsf(value[i]) + fabsf(least)) : 0.0f))
+      open |= 1u << i;
+  if (!close) open = 0;
+  double d1 = -INFINITY, d2 = -INFINITY;
+#pragma unroll 1
+  for (; __ballot(open != 0) != 0; open &= open - 1)
+    if (open != 0) merge_two(d1, d2, exact(sub * C + __builtin_ctz(open), sum), (double)-INFINITY);
+#pragma unroll 1
+  for (int off = 1; off < 1 << shift; off *= 2) merge_two(d1, d2, __shfl_xor(d1, off, L), __shfl_xor(d2, off, L));
+  const uint64_t v = order_of(two ? d1 + d2 : d1);
+  const int g = sub >> shift;
+  wave_sync();
+  if (g << shift == sub) m.key[g] = v;
+  wave_sync();
+  int better = 0;
+#pragma unroll 1
+  for (int i = 0; i < opt.n_groups; ++i) better += m.key[i] > v || (m.key[i] == v && i < g);
+  wave_sync();
+  return close ? better < opt.topk_groups : stays;
 }
 
 // The top_k experts of the largest keys (0: none) into m.pick, their values into
@@ -555,14 +585,16 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
       double sum = 0.0;
       if (softmax) {
         float* const values = reinterpret_cast<float*>(m.key);
+        float again[C];  // (the row's logits: kept, they would cost the main path registers)
+        load_run<T, C>(row, sub * C, n_experts, vec, -INFINITY, again);
         wave_sync();
 #pragma unroll
-        for (int i = 0; i < C; ++i) values[sub * C + i] = l[i];
+        for (int i = 0; i < C; ++i) values[sub * C + i] = again[i];
         wave_sync();
 #pragma unroll 1
         for (int i = 0; i < C; ++i) {
           const float x = values[sub * C + i];
-          if (x != -INFINITY) sum += exp((double)x - (double)mx);
+          if (x != -INFINITY) sum += exp64((double)x - (double)mx);
         }
         sum = lanes_sum<L>(sum);
         wave_sync();
@@ -578,13 +610,9 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
     for (int i = 0; i < C; ++i) key[i] = sub * C + i >= n_experts ? 0 : key_of(value[i], i);
     uint32_t in = ~0u;  // the lane's experts in groups that stay
     if constexpr (kGroups) {
-      bool again = opt.n_groups <= L;
       if (shape.shift >= 0) {
-        bool close = false;
-        in = group_stays<L, C>(value, tol, bias != nullptr, sub, opt, shape.shift, score, close) ? ~0u : 0u;
-        again = __ballot(close && on) != 0;
-      }
-      if (again) {
+        in = group_stays<L, C>(value, tol, bias != nullptr, sub, opt, shape.shift, on, m, score, sum64, exact) ? ~0u : 0u;
+      } else if (opt.n_groups <= L) {
         float worth[C];  // what the groups go by
 #pragma unroll
         for (int i = 0; i < C; ++i)
@@ -624,6 +652,13 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
         const int e0 = look(top_k - 1, l0, b0);
         const float v0 = score(l0) + b0;
         const uint32_t k0 = key_of(a, 15);
+        float ls[C], bs[C];
+        load_run<T, C>(row, sub * C, n_experts, vec, -INFINITY, ls);
+        if (bias != nullptr)
+          load_run<float, C>(bias, sub * C, n_experts, vec_bias, 0.0f, bs);
+        else
+#pragma unroll
+          for (int i = 0; i < C; ++i) bs[i] = 0.0f;
         uint32_t open = 0;  // the lane's experts that may be among the chosen
 #pragma unroll
         for (int i = 0; i < C; ++i) {
@@ -631,7 +666,7 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
           const uint32_t ki = stays ? key_of(value[i], 15) : kOffKey;
           const bool beside = apart(a, value_of(ki)), left = ki < k0 || (ki == k0 && sub * C + i > e0);
           if (sub * C + i < n_experts && (ki >= k0 || beside)) open |= 1u << i;
-          close |= beside && left && (l[i] != l0 || b[i] != b0) && swapped(v0, value[i]);
+          close |= beside && left && (ls[i] != l0 || bs[i] != b0) && swapped(v0, value[i]);
         }
         const bool again = lanes_of<L>(close && on) != 0;
         if (__ballot(again) != 0) {
