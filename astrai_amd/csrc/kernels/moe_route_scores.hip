@@ -30,9 +30,9 @@
 // maximum and a minimum. A pick is a maximum over the lanes' first ones (DPP, no LDS)
 // and the first lane that has it; that lane notes the expert and moves its list up.
 // Groups of whole lanes are valued and picked in registers alike.
-// Bound by the instructions (1370 of the vector units a wave of four tokens), not by the
-// logits' bytes: 16384 tokens of 256 experts in 8 groups, sigmoid scores with a bias, 19
-// to 22 us (the logits' 17 MB: 3.3), 12 of them without the near ties, which a wave
+// Bound by the instructions (1380 of the vector units a wave of four tokens), not by the
+// logits' bytes: 16384 tokens of 256 experts in 8 groups, sigmoid scores with a bias, 17
+// to 20 us (the logits' 17 MB: 3.3), 12 of them without the near ties, which a wave
 // settles while the others are done; softmax without groups and bias 10.
 #include "moe_common.h"
 #include "moe_gemm.h"
@@ -867,8 +867,8 @@ int launch_scores(const void* logits, const float* bias, const astrai_moe_routin
   launch_scores_cfg<T, W, L, C>(logits, bias, opt, n_tokens, n_experts, top_k, n_shared, topk_idx, topk_w,      \
                                 chunk_hist, list, s)
   // As many lanes as groups, more than 64 of which are for choose_slowly. (16384 tokens, us,
-  // 128 experts in 32 groups by 16 lanes, so choose_slowly, 82, by 32 lanes 32; 256 in 64
-  // groups by 16 lanes 126, by 64 lanes 94.)
+  // 128 experts in 32 groups by 16 lanes, so choose_slowly, 82, by 32 lanes 31; 256 in 64
+  // groups by 16 lanes 126, by 64 lanes 92.)
   const bool few = opt.n_groups <= 16;
   if (n_experts <= 32 && few)
     ROUTE_CASE(16, 2);

@@ -59,6 +59,28 @@ def test_route_scores_refuses_before_any_device_work():
     _refused(lib.astrai_moe_balance_bias(None, 16, 8, 0.1, 16, None), "null buffer")
 
 
+def test_forward_scores_refuses_before_any_device_work():
+    lib = loader.library()
+    sizes = (4, 8, 2, 1, 64, 64)
+    need = lib.astrai_moe_forward_workspace_bytes(*sizes, BF16, 0)
+    assert need > 0
+
+    def call(routing, ldtype=F32, sizes=sizes, ws=256, nbytes=need, packed=None, x=16):
+        return lib.astrai_moe_forward_scores(x, 16, ldtype, None, routing, 16, 16, 16, packed, None, BF16, *sizes, ws, nbytes,
+                                             16, None)
+
+    _refused(call(None), "null routing")
+    _refused(call(_routing(score=5)), "score")
+    _refused(call(_routing(n_groups=3)), "divide")
+    _refused(call(_routing(), ldtype=7), "dtype")
+    _refused(call(_routing(scale=math.inf)), "finite")
+    _refused(call(_routing(), packed=16), "packed")
+    _refused(call(_routing(), x=None), "null buffer")
+    _refused(call(_routing(), nbytes=need - 1), "")
+    _refused(call(_routing(), sizes=(4, 8, 9, 1, 64, 64)), "top_k")
+    assert call(_routing(), sizes=(0, 8, 2, 1, 64, 64)) == 0
+
+
 def test_int8_refuses_before_any_device_work():
     lib = loader.library()
     assert [lib.astrai_moe_int8_row_bytes(k) for k in (0, 1, 16, 17)] == [0, 16, 16, 32]
