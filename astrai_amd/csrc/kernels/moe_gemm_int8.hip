@@ -1324,7 +1324,11 @@ bool int8_quantises(int64_t most_rows, int64_t k, int64_t row_tiles, int64_t n, 
 // the bf16 ones, but for more than 32 rows of one expert only where a round holds all
 // the column tiles, each of which stages every row again (us a product with / without
 // them: 4096 to 14336, 448 tiles, 40 rows 31.9 / 25.5, 100 38.2 / 26.4; 14336 to 4096,
-// 128 tiles, 40 25.5 / 63.5, 128 34.7 / 64.7; 2048 to 5632, 176 tiles, 64 11.5 / 14.6).
+// 128 tiles, 40 25.5 / 63.5, 128 34.7 / 64.7; 2048 to 5632, 176 tiles, 64 11.5 / 14.6);
+// and in 64-row lists where a round holds the tiles of all runs of 64 rows (512 to 512, 500
+// rows 7.2 / 8.5; 1000 to 2664, 130 rows 8.9 / 12.2; 4096 to 1024, 333 rows 13.7 / 22.6;
+// in two rounds 1000 to 2664, 333 rows 12.5 / 12.7, 512 to 2048 9.4 / 8.6, 1024 to 4096
+// 15.5 / 11.9).
 // And routed rows of short products only where two rounds hold their column tiles:
 // with fewer than kFewMinSteps K steps, of which a wave takes every fourth, a tile's
 // sums cost more than its loads (us a layer with / without: 64 experts, top-6 and a
@@ -1336,6 +1340,7 @@ bool int8_few_rows(const RowCounts& rows, int block_m, int64_t kp, int64_t n, bo
   const double cols = (double)ceil_div(n, gate_up ? 16 : 32);
   if (rows.dense()) {
     if (rows.exact_rows > 32 && cols > cu_count()) return false;
+    if (block_m == kMfmaMidBM && ceil_div(rows.exact_rows, kMfmaMidBM) * cols <= cu_count()) return true;
   } else if (ceil_div(kp, kRowBytes) < kFewMinSteps) {
     const double e = rows.experts, live = e > 0 ? e * (1.0 - std::pow(1.0 - 1.0 / e, (double)rows.rows)) : 0.0;
     if ((live + rows.exact) * cols > 2.0 * cu_count()) return false;
