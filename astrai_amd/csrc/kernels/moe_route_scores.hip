@@ -389,7 +389,8 @@ __device__ __forceinline__ bool group_stays(const float (&value)[C], float tol, 
   }
   if (tol == 0.0f) return stays;
   const float next = float_of(max(lanes_max<L>(mine), bits_of(-INFINITY)));
-  const bool close = on && next > -INFINITY && float_of(last) - next <= 2.0f * tol + 4.0f * kTolAdd * lanes_max<L>(size);
+  const float sizes = lanes_max<L>(size);
+  const bool close = on && next > -INFINITY && float_of(last) - next <= 2.0f * tol + 4.0f * kTolAdd * sizes;
   if (__ballot(close) == 0) return stays;
   const double sum = sum64();
   uint32_t open = 0;  // (logits are exact)

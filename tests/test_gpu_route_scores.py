@@ -334,6 +334,40 @@ def test_large_biases_that_cancel_in_a_group(gpu):
         _check_route(ops.moe_route_scores(logits, 4, routing, bias), logits, 4, routing, bias, torch.float32)
 
 
+def test_captured_training_side_replays(gpu):
+    """Routing, gradient, load and the bias's step in one graph: every replay on new
+    logits as the eager calls, with eager work of other sizes in between."""
+    routing = ops.Routing("sigmoid", 8, 4, 2, True, 2.5)
+    gen = torch.Generator().manual_seed(3)
+    logits, bias = torch.randn(700, 128, generator=gen).to(gpu), torch.zeros(128, device=gpu)
+    dw = torch.randn(700, 8, generator=gen).to(gpu)
+
+    def step(b):
+        r = ops.moe_route_scores(logits, 8, routing, b)
+        g = ops.moe_route_scores_grad(logits, r.topk_idx, r.topk_w, dw, routing)
+        load = ops.moe_expert_load(r.chunk_hist)
+        return (*r, g, load, ops.moe_balance_bias(b, load, 0.01, out=b))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        step(bias.clone())
+        with torch.cuda.graph(graph, stream=stream):
+            got = step(bias)
+    torch.cuda.current_stream().wait_stream(stream)
+    eager = torch.zeros(128, device=gpu)
+    for i in range(4):
+        logits.copy_(torch.randn(700, 128, generator=gen))
+        graph.replay()
+        want = step(eager)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i
+        ops.moe_route_scores(torch.randn(50 + i, 60, device=gpu), 4)
+        torch.cuda.synchronize()
+    assert (bias != 0).any()
+
+
 def test_no_tokens(gpu):
     r = ops.moe_route_scores(torch.empty(0, 64, device=gpu), 4)
     assert r.topk_idx.shape == (0, 4) and r.chunk_hist.shape == (0, 64)
