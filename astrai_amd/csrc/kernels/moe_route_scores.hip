@@ -504,9 +504,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // exp on the hardware's exponential: off by |x| 2^-24 + 2^-23 of its value.
 __device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// Score of an expert in 32 bits (softmax: with the row's maximum and 1 / sum).
-__device__ __forceinline__ float score32(float l, bool softmax, float mx, float inv) {
-  return softmax ? expf(l - mx) * inv : 1.0f / (1.0f + expf(-l));
+// Score of an expert in 32 bits over e^base (a softmax's without 1 / sum; a sigmoid's base
+// is at most 0): renormalised weights take the largest chosen logit, so that scores below
+// every float still have their share. What 64 bits hold as 0 is 0.
+constexpr float kLeastLog = -708.0f;
+__device__ __forceinline__ float score32(float l, bool softmax, float base, float mx) {
+  if (softmax) return l - mx < kLeastLog ? 0.0f : expf(l - base);
+  const float d = 1.0f / (1.0f + expf(-fabsf(l)));
+  return l >= 0.0f ? d : l < kLeastLog ? 0.0f : expf(l - base) * d;
 }
 
 template <int L, bool kList>
@@ -691,17 +696,25 @@ __global__ __launch_bounds__((score_threads<L, kList>()), 4) void route_scores_k
     }
     // the weights, slots k = sub, sub + L, ...
     constexpr int SLOTS = ASTRAI_MOE_MAX_TOPK > L ? ASTRAI_MOE_MAX_TOPK / L : 1;
-    float v[SLOTS], total = 0.0f;
+    float v[SLOTS], total = 0.0f, best = -INFINITY;
     int e[SLOTS];
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
       const int k = sub + i * L;
-      v[i] = 0.0f, e[i] = 0;
+      v[i] = -INFINITY, e[i] = 0;
       if (on && k < top_k) {
         e[i] = m.pick[k];
-        const float got = m.score[k];  // NaN: the row holds no number; -inf: no live expert
-        v[i] = got == -INFINITY ? 0.0f : got != got ? got : score32(Elem<T>::to_f32(logits[t * n_experts + e[i]]), softmax, mx, inv);
+        v[i] = m.score[k];  // NaN: the row holds no number; -inf: no live expert
+        if (v[i] > -INFINITY) v[i] = Elem<T>::to_f32(logits[t * n_experts + e[i]]);
       }
+      best = fmaxf(best, v[i]);
+    }
+    best = lanes_max<L>(best);
+    const float base = opt.renormalise ? (softmax ? best : fminf(best, 0.0f)) : softmax ? mx : 0.0f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const float s = score32(v[i], softmax, base, mx);
+      v[i] = v[i] == -INFINITY ? 0.0f : v[i] != v[i] ? v[i] : softmax && !opt.renormalise ? s * inv : s;
       total += v[i];
     }
     total = lanes_sum<L>(total);
@@ -779,8 +792,13 @@ __global__ __launch_bounds__(256) void route_scores_grad_kernel(
     }
   } else {
     // 1 - s(l) = s(-l), without the cancellation
+    // (over e^base, as the weights)
+    float base = renorm ? chosen : 0.0f;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) base = fmaxf(base, __shfl_xor(base, off, 64));
+    base = fminf(base, 0.0f);
     const float e = expf(-fabsf(chosen)), d = 1.0f / (1.0f + e);
-    s = chosen >= 0.0f ? d : e * d;
+    s = chosen >= 0.0f ? d : chosen == -INFINITY ? 0.0f : expf(chosen - base) * d;
     against = chosen >= 0.0f ? e * d : d;
   }
   float at_chosen, dot = 0.0f;

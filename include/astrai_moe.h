@@ -533,8 +533,8 @@ int astrai_moe_gemm_wgrad(const void* a, const void* b,
  *   topk_idx: the top_k largest c among these, descending (ties: the lower
  *     expert); slots without a c above -inf left take the lowest experts not yet
  *     chosen and weight 0
- *   topk_w = scale s / S over the chosen s, S their sum (0 where S = 0), or with
- *     renormalise 0 scale s; rounded once to weight_dtype
+ *   topk_w = scale s / S over the chosen s, S their sum (0 where S = 0 in 64 bits),
+ *     or with renormalise 0 scale s; rounded once to weight_dtype
  * Without a bias, c is ordered as its logits are (also where scores in 64 bits are
  * equal); with one, and for group values of two scores, in 64 bits. A row with a NaN
  * logit (softmax: or +inf) has experts 0 .. top_k - 1 and NaN weights.

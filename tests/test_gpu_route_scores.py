@@ -320,6 +320,30 @@ def test_logits_at_the_ends_of_their_range(gpu, score):
         assert (g == 0).all()
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_scores_below_every_float_keep_their_share(gpu, score):
+    """Chosen experts (by the bias alone) whose scores are 1e-45 to 1e-275: the weights
+    and their gradient are those of 64 bits."""
+    gen = torch.Generator().manual_seed(9)
+    logits = torch.randn(100, 64, generator=gen)
+    logits[:, 10:14] = -torch.rand(100, 1, generator=gen) * 500.0 - 120.0 + torch.randn(100, 4, generator=gen) * 5.0
+    logits, bias = logits.to(gpu), torch.zeros(64, device=gpu)
+    bias[10:14] = torch.tensor([40.0, 30.0, 20.0, 10.0], device=gpu)
+    routing = ops.Routing(score, scale=2.5)
+    r = ops.moe_route_scores(logits, 4, routing, bias)
+    _check_route(r, logits, 4, routing, bias, torch.float32)
+    dw = torch.randn(100, 4, generator=gen).to(gpu)
+    got = ops.moe_route_scores_grad(logits, r.topk_idx, r.topk_w, dw, routing)
+    l = logits.double().gather(1, r.topk_idx.long())
+    w = torch.softmax(l, -1)  # (a sigmoid of these is exp(l), and 1 - s is 1)
+    terms = w.unsqueeze(2) * w.unsqueeze(1) * (dw.double().unsqueeze(2) - dw.double().unsqueeze(1)) * 2.5
+    err = (got.gather(1, r.topk_idx.long()).double() - terms.sum(2)).abs()
+    # a difference d of logits, at most 40, is rounded by |d| 2^-24 < 2^-18, which is the
+    # relative error of its exponential; r is a quotient of two such (2^-17), a term a
+    # product of two r
+    assert (err <= 2.0 ** -15 * terms.abs().sum(2) + 1e-38).all()
+
+
 def test_large_biases_that_cancel_in_a_group(gpu):
     """Group values whose parts are far larger than their sums: rounded in 32 bits they
     lose what tells the groups apart."""
